@@ -27,6 +27,9 @@
 #include "rotq_tc.cuh"
 #include "llama_ops.cuh"
 #include "scatter_block.cuh"
+#include "kv4.cuh"
+#include "kv4_attention.cuh"
+#include "token_logprobs.cuh"
 
 namespace {
 
@@ -448,6 +451,81 @@ int dispatch_split(const CUtensorMap& tmP, const CUtensorMap& tmQ, const dscq::G
   return gp.splits > 1 ? launch_gemm_kernel<BN, SWAP, true>(tmP, tmQ, gp, stream)
                        : launch_gemm_kernel<BN, SWAP, false>(tmP, tmQ, gp, stream);
 }
+
+}  // namespace
+
+// ------------------------------------------------------------------ 4-bit paged cache
+namespace {
+
+// The device form of a batch, after checking what the host can see of it.
+int kv4_batch(const dscq_kv4_batch* b, int64_t T, dscq::Kv4Batch* out) {
+  DSCQ_REQUIRE(b != nullptr, "batch must not be null");
+  DSCQ_REQUIRE(b->k_codes && b->k_affine && b->v_codes && b->v_affine, "cache buffers must not be null");
+  DSCQ_REQUIRE(b->head_dim == 64 || b->head_dim == 128, "head_dim must be 64 or 128");
+  DSCQ_REQUIRE(b->dtype == DSCQ_BF16 || b->dtype == DSCQ_F16, "the cache's type must be bf16 or f16");
+  DSCQ_REQUIRE(b->page_size >= 16 && b->page_size <= 1024 && (b->page_size & (b->page_size - 1)) == 0,
+               "page_size must be a power of two from 16 to 1024");
+  DSCQ_REQUIRE(b->kv_heads >= 1 && b->kv_heads <= 4096 && b->pages >= 1 && b->pages < (int64_t(1) << 31),
+               "need 1 <= kv_heads <= 4096 and 1 <= pages < 2^31");
+  DSCQ_REQUIRE(b->seqs >= 0 && b->seqs < (int64_t(1) << 30), "invalid number of sequences");
+  DSCQ_REQUIRE(b->seqs == 0 || (b->page_table && b->q_start && b->lengths),
+               "page_table, q_start and lengths must not be null");
+  DSCQ_REQUIRE(b->max_pages >= 0 && b->ld_table >= b->max_pages && b->max_pages * b->page_size < (int64_t(1) << 31),
+               "need ld_table >= max_pages and max_pages * page_size < 2^31");
+  DSCQ_REQUIRE(T >= 0 && T < (int64_t(1) << 31), "need 0 <= T < 2^31");
+  DSCQ_REQUIRE(aligned(b->k_codes, 16) && aligned(b->v_codes, 16) && aligned(b->k_affine, 16) &&
+                   aligned(b->v_affine, 16),
+               "cache buffers must be 16-byte aligned");
+  out->kc = static_cast<uint8_t*>(b->k_codes);
+  out->vc = static_cast<uint8_t*>(b->v_codes);
+  out->ka = static_cast<uint32_t*>(b->k_affine);
+  out->va = static_cast<uint32_t*>(b->v_affine);
+  out->table = b->page_table;
+  out->q_start = b->q_start;
+  out->lengths = b->lengths;
+  out->pages = b->pages;
+  out->ld_table = b->ld_table;
+  out->B = static_cast<int>(b->seqs);
+  out->P = static_cast<int>(b->max_pages);
+  out->hk = b->kv_heads;
+  out->ps_log2 = 0;
+  while ((1 << out->ps_log2) < b->page_size) ++out->ps_log2;
+  return DSCQ_OK;
+}
+
+bool rows_ok(const void* p, int64_t st, int64_t sh) { return p && aligned(p, 16) && st % 8 == 0 && sh % 8 == 0; }
+
+template <typename T, int D>
+cudaError_t launch_kv4_append(const dscq::Kv4AppendParams& p, bool f32, cudaStream_t st) {
+  const int rows = p.hq + 2 * p.b.hk, per = dscq::Kv4Rows<D>::kPerCta;
+  const dim3 grid(static_cast<unsigned>(p.T), static_cast<unsigned>((rows + per - 1) / per));
+  if (f32)
+    dscq::kv4_append_kernel<T, D, true><<<grid, 256, 0, st>>>(p);
+  else
+    dscq::kv4_append_kernel<T, D, false><<<grid, 256, 0, st>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename T, int D>
+cudaError_t launch_kv4_read(const dscq::Kv4Batch& b, int64_t rows, void* k, void* v, cudaStream_t st) {
+  const int per = dscq::Kv4Rows<D>::kPerCta;
+  const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>((2 * b.hk + per - 1) / per));
+  dscq::kv4_read_kernel<T, D><<<grid, 256, 0, st>>>(b, static_cast<T*>(k), static_cast<T*>(v));
+  return cudaGetLastError();
+}
+
+template <typename T, int D>
+cudaError_t launch_kv4_attention(const dscq::Kv4AttnParams& p, cudaStream_t st) {
+  const int64_t items = static_cast<int64_t>(p.T) * p.hq;
+  dscq::kv4_attention_rows<T, D><<<static_cast<unsigned>((items + 3) / 4), 128, 0, st>>>(p);
+  return cudaGetLastError();
+}
+
+// f.template operator()<T, D>() for the cache's type and head dimension.
+#define DSCQ_KV4_DISPATCH(batch, call)                                       \
+  ((batch)->dtype == DSCQ_BF16                                               \
+       ? ((batch)->head_dim == 64 ? call(__nv_bfloat16, 64) : call(__nv_bfloat16, 128)) \
+       : ((batch)->head_dim == 64 ? call(__half, 64) : call(__half, 128)))
 
 }  // namespace
 
@@ -1045,6 +1123,99 @@ int dscq_silu_mul(const void* g, const void* u, int64_t n, void* y, void* stream
       static_cast<const __nv_bfloat16*>(g), static_cast<const __nv_bfloat16*>(u), static_cast<__nv_bfloat16*>(y), n);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "launch silu_mul");
+  return DSCQ_OK;
+}
+
+int dscq_kv4_append(const dscq_kv4_batch* batch, const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                    int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h,
+                    int64_t T, int q_heads, const void* cos_t, const void* sin_t, int table_dtype, int64_t table_rows,
+                    void* q_out, void* stream) {
+  dscq::Kv4AppendParams p{};
+  int st = kv4_batch(batch, T, &p.b);
+  if (st) return st;
+  DSCQ_REQUIRE(q_heads >= 1 && q_heads <= 65536, "need 1 <= q_heads <= 65536");
+  DSCQ_REQUIRE(table_dtype == batch->dtype || table_dtype == DSCQ_F32, "cos / sin must have the cache's type or be f32");
+  DSCQ_REQUIRE(table_rows >= 0 && table_rows < (int64_t(1) << 31), "invalid number of table rows");
+  if (T == 0) return DSCQ_OK;
+  DSCQ_REQUIRE(rows_ok(q, q_stride_t, q_stride_h) && rows_ok(k, k_stride_t, k_stride_h) &&
+                   rows_ok(v, v_stride_t, v_stride_h) && q_out && aligned(q_out, 16),
+               "q, k, v and q_out must be 16-byte aligned with strides that are multiples of 8");
+  DSCQ_REQUIRE(cos_t && sin_t && aligned(cos_t, 16) && aligned(sin_t, 16), "cos and sin must be 16-byte aligned");
+  st = check_device(nullptr);
+  if (st) return st;
+  p.q = q, p.k = k, p.v = v, p.cos = cos_t, p.sin = sin_t, p.q_out = q_out;
+  p.q_t = q_stride_t, p.q_h = q_stride_h, p.k_t = k_stride_t, p.k_h = k_stride_h, p.v_t = v_stride_t, p.v_h = v_stride_h;
+  p.T = static_cast<int>(T), p.hq = q_heads, p.table_rows = static_cast<int>(table_rows);
+  const bool f32 = table_dtype == DSCQ_F32;
+#define DSCQ_CALL(TY, D) launch_kv4_append<TY, D>(p, f32, static_cast<cudaStream_t>(stream))
+  cudaError_t e = DSCQ_KV4_DISPATCH(batch, DSCQ_CALL);
+#undef DSCQ_CALL
+  if (e != cudaSuccess) return cuda_fail(e, "launch kv4_append");
+  return DSCQ_OK;
+}
+
+int dscq_kv4_read(const dscq_kv4_batch* batch, int64_t T, void* k_out, void* v_out, void* stream) {
+  dscq::Kv4Batch b{};
+  int st = kv4_batch(batch, T, &b);
+  if (st) return st;
+  if (T == 0) return DSCQ_OK;
+  DSCQ_REQUIRE(k_out && v_out && aligned(k_out, 16) && aligned(v_out, 16), "outputs must be 16-byte aligned");
+  st = check_device(nullptr);
+  if (st) return st;
+#define DSCQ_CALL(TY, D) launch_kv4_read<TY, D>(b, T, k_out, v_out, static_cast<cudaStream_t>(stream))
+  cudaError_t e = DSCQ_KV4_DISPATCH(batch, DSCQ_CALL);
+#undef DSCQ_CALL
+  if (e != cudaSuccess) return cuda_fail(e, "launch kv4_read");
+  return DSCQ_OK;
+}
+
+int dscq_kv4_attention(const dscq_kv4_batch* batch, const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t T,
+                       int q_heads, float scale, void* out, void* stream) {
+  dscq::Kv4AttnParams p{};
+  int st = kv4_batch(batch, T, &p.b);
+  if (st) return st;
+  DSCQ_REQUIRE(q_heads >= 1 && q_heads <= 65536 && q_heads % batch->kv_heads == 0,
+               "q_heads must be a multiple of kv_heads");
+  DSCQ_REQUIRE(std::isfinite(scale), "scale must be finite");
+  if (T == 0) return DSCQ_OK;
+  DSCQ_REQUIRE(rows_ok(q, q_stride_t, q_stride_h) && out && aligned(out, 16),
+               "q and out must be 16-byte aligned with strides that are multiples of 8");
+  st = check_device(nullptr);
+  if (st) return st;
+  p.q = q, p.out = out, p.q_t = q_stride_t, p.q_h = q_stride_h;
+  p.T = static_cast<int>(T), p.hq = q_heads, p.group = q_heads / batch->kv_heads;
+  p.scale_log2 = scale * 1.4426950408889634f;
+#define DSCQ_CALL(TY, D) launch_kv4_attention<TY, D>(p, static_cast<cudaStream_t>(stream))
+  cudaError_t e = DSCQ_KV4_DISPATCH(batch, DSCQ_CALL);
+#undef DSCQ_CALL
+  if (e != cudaSuccess) return cuda_fail(e, "launch kv4_attention");
+  return DSCQ_OK;
+}
+
+int dscq_token_logprobs(const void* logits, int x_dtype, int64_t rows, int64_t V, int64_t ld, const int64_t* targets,
+                        int k, float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids, void* stream) {
+  DSCQ_REQUIRE(x_dtype == DSCQ_BF16 || x_dtype == DSCQ_F16 || x_dtype == DSCQ_F32, "logits must be bf16, f16 or f32");
+  DSCQ_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) && V >= 1 && V <= (int64_t(1) << 24) && ld >= V,
+               "need 0 <= rows < 2^31, 1 <= V <= 2^24 and ld >= V");
+  DSCQ_REQUIRE(k >= 0 && k <= 64 && k <= V, "need 0 <= k <= 64 and k <= V");
+  if (rows == 0) return DSCQ_OK;
+  DSCQ_REQUIRE(logits && targets && logprobs && entropy && (k == 0 || (top_logprobs && top_ids)),
+               "buffers must not be null");
+  DSCQ_REQUIRE(aligned(logits, x_dtype == DSCQ_F32 ? 4 : 2), "logits must be aligned to their type");
+  int st = check_device(nullptr);
+  if (st) return st;
+  dscq::LogprobParams p{logits, targets, logprobs, entropy, top_logprobs, top_ids,
+                        ld,     static_cast<int>(rows), static_cast<int>(V), k};
+  cudaStream_t cst = static_cast<cudaStream_t>(stream);
+  const unsigned grid = static_cast<unsigned>(rows);
+  if (x_dtype == DSCQ_BF16)
+    dscq::logprob_rows<__nv_bfloat16><<<grid, 256, 0, cst>>>(p);
+  else if (x_dtype == DSCQ_F16)
+    dscq::logprob_rows<__half><<<grid, 256, 0, cst>>>(p);
+  else
+    dscq::logprob_rows<float><<<grid, 256, 0, cst>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "launch token_logprobs");
   return DSCQ_OK;
 }
 

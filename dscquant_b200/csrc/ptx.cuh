@@ -29,6 +29,7 @@ namespace dscq {
 enum : uint32_t {
   kStatusWaitTimeout = 1u << 0,   // an mbarrier / cluster wait expired
   kStatusBadLaunch = 1u << 1,     // kernel saw inconsistent launch geometry
+  kStatusBadIndex = 1u << 2,      // a page, length or token id in device memory was out of range (skipped)
 };
 
 __device__ uint32_t g_status;

@@ -19,6 +19,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
+from .kvcache import PagedKV4
 
 _DT = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float32: _lib.F32}
 _MODES = {"act_sym": _lib.ACT_SYM, "weight_sym": _lib.WEIGHT_SYM, "act_asym": _lib.ACT_ASYM,
@@ -395,3 +396,156 @@ def silu_mul(g: torch.Tensor, u: torch.Tensor) -> torch.Tensor:
     y = torch.empty_like(g)
     _lib.check(_lib.load().dscq_silu_mul(_ptr(g), _ptr(u), g.numel(), _ptr(y), _stream(g.device)), "silu_mul")
     return y
+
+
+# ------------------------------------------------------------------ generation: 4-bit paged cache, scoring
+def _no_grad_inputs(*tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError("this operator has no backward pass: call it under torch.no_grad()")
+
+
+def _kv4_batch(cache: PagedKV4, page_table: torch.Tensor, q_start: torch.Tensor, lengths: torch.Tensor):
+    """The dscq_kv4_batch of a call, after the checks every cache operator makes."""
+    dev = cache.device
+    for name, t in (("page_table", page_table), ("q_start", q_start), ("lengths", lengths)):
+        if t.dtype != torch.int32 or t.device != dev:
+            raise RuntimeError(f"{name} must be an int32 tensor on {dev}")
+    B = lengths.numel()
+    if lengths.dim() != 1 or q_start.dim() != 1 or q_start.numel() != B + 1:
+        raise RuntimeError("need lengths [B] and q_start [B + 1]")
+    if page_table.dim() != 2 or page_table.shape[0] != B:
+        raise RuntimeError("page_table must be [B, pages]")
+    if (B > 1 and (lengths.stride(0) != 1 or page_table.stride(0) < page_table.shape[1])) or \
+            (B and q_start.stride(0) != 1) or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise RuntimeError("page_table rows, q_start and lengths must be contiguous")
+    pages, hk, ps, half = cache.k_codes.shape
+    P = page_table.shape[1]
+    return _lib.Kv4Batch(cache.k_codes.data_ptr(), cache.k_affine.data_ptr(), cache.v_codes.data_ptr(),
+                         cache.v_affine.data_ptr(), pages, hk, ps, half * 2, _DT[cache.dtype],
+                         page_table.data_ptr(), max(page_table.stride(0), P), P, q_start.data_ptr(),
+                         lengths.data_ptr(), B)
+
+
+def _kv4_rows(cache: PagedKV4, name: str, t: torch.Tensor, T: int, heads: int | None) -> None:
+    if t.dim() != 3 or t.shape[0] != T or t.shape[2] != cache.head_dim or (heads is not None and t.shape[1] != heads):
+        raise RuntimeError(f"{name} must be [{T}, {heads or 'heads'}, {cache.head_dim}]")
+    if t.dtype != cache.dtype or t.device != cache.device:
+        raise RuntimeError(f"{name} must be a {cache.dtype} tensor on {cache.device}")
+    if t.numel() and (t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16):
+        raise RuntimeError(f"{name} needs unit stride in its last dimension, other strides a multiple of 8 and "
+                           "16-byte alignment")
+
+
+def kv4_append(cache: PagedKV4, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
+               sin: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor,
+               lengths: torch.Tensor) -> torch.Tensor:
+    """Rotates q and k by position (rotate-half form), writes k and v to the cache as 4-bit rows and returns
+    the rotated queries [T, q_heads, D]; one kernel.
+
+    q [T, q_heads, D], k and v [T, kv_heads, D] of the cache's type (views with strides are fine). Rows
+    q_start[b] .. q_start[b+1]-1 are the newest tokens of sequence b; lengths[b] counts its tokens including
+    them, so row i of n stands at position lengths[b] - n + i, and page_table[b, position // page_size] is its
+    page. cos / sin [positions, D] are tables by position, of the cache's type or float32. Rows of no sequence
+    (behind the last one) give zero queries and write nothing. No two rows of a call may share a slot. A
+    position or page out of range is left out and raises bit 2 of `device_status`."""
+    if q.dim() != 3:
+        raise RuntimeError("q must be [T, heads, D]")
+    T, dev = q.shape[0], cache.device
+    for name, t, heads in (("q", q, None), ("k", k, cache.kv_heads), ("v", v, cache.kv_heads)):
+        _kv4_rows(cache, name, t, T, heads)
+    _no_grad_inputs(q, k, v)
+    for name, t in (("cos", cos), ("sin", sin)):
+        if t.dim() != 2 or t.shape != cos.shape or t.shape[1] != cache.head_dim or not t.is_contiguous():
+            raise RuntimeError(f"{name} must be a contiguous [positions, {cache.head_dim}] table")
+        if t.dtype not in (cache.dtype, torch.float32) or t.dtype != cos.dtype or t.device != dev:
+            raise RuntimeError(f"cos and sin must both be {cache.dtype} or both float32, on {dev}")
+    batch = _kv4_batch(cache, page_table, q_start, lengths)
+    with torch.cuda.device(dev):
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        rc = _lib.load().dscq_kv4_append(batch, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
+                                         k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), T, q.shape[1],
+                                         cos.data_ptr(), sin.data_ptr(), _DT[cos.dtype], cos.shape[0],
+                                         out.data_ptr(), _stream(dev))
+    _lib.check(rc, "kv4_append")
+    return out
+
+
+def kv4_read(cache: PagedKV4, page_table: torch.Tensor, q_start: torch.Tensor, lengths: torch.Tensor,
+             rows: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values the cache holds for `rows` rows of the token axis (the same batch description as
+    kv4_append), [rows, kv_heads, D] each; zero for rows of no sequence. With q_start counting every token of
+    each sequence it reads whole sequences back."""
+    dev = cache.device
+    batch = _kv4_batch(cache, page_table, q_start, lengths)
+    with torch.cuda.device(dev):
+        k = torch.empty((rows, cache.kv_heads, cache.head_dim), dtype=cache.dtype, device=dev)
+        v = torch.empty_like(k)
+        rc = _lib.load().dscq_kv4_read(batch, rows, k.data_ptr(), v.data_ptr(), _stream(dev))
+    _lib.check(rc, "kv4_read")
+    return k, v
+
+
+def kv4_attention(cache: PagedKV4, q: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor,
+                  lengths: torch.Tensor, *, scale: float | None = None, max_q: int | None = None) -> torch.Tensor:
+    """Causal attention of the newest tokens of each sequence over its cached keys and values, [T, q_heads, D].
+
+    q [T, q_heads, D] of the cache's type, already rotated (kv4_append's result); the batch is described as for
+    kv4_append, whose rows it must already hold. Query head h reads key head h // (q_heads // kv_heads), a row
+    at position p the positions 0 .. p. `scale` defaults to D ** -0.5. `max_q` says how many rows the longest
+    sequence has in this call (default T). Rows of no sequence, and rows that see no key, are zero."""
+    if q.dim() != 3:
+        raise RuntimeError("q must be [T, heads, D]")
+    T, dev = q.shape[0], cache.device
+    _kv4_rows(cache, "q", q, T, None)
+    _no_grad_inputs(q)
+    if q.shape[1] % cache.kv_heads or q.shape[1] == 0:
+        raise RuntimeError("q's heads must be a multiple of the cache's")
+    batch = _kv4_batch(cache, page_table, q_start, lengths)
+    with torch.cuda.device(dev):
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        rc = _lib.load().dscq_kv4_attention(batch, q.data_ptr(), q.stride(0), q.stride(1), T, q.shape[1],
+                                            cache.head_dim ** -0.5 if scale is None else float(scale),
+                                            out.data_ptr(), _stream(dev))
+    _lib.check(rc, "kv4_attention")
+    return out
+
+
+@dataclass
+class TokenLogprobs:
+    logprobs: torch.Tensor      # [rows] f32: log probability of the given token
+    entropy: torch.Tensor       # [rows] f32, in nats
+    top_logprobs: torch.Tensor  # [rows, top_k] f32, larger first
+    top_ids: torch.Tensor       # [rows, top_k] i64
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) -> TokenLogprobs:
+    """Log probability of targets[r] under softmax(logits[r]), the entropy of that distribution and its top_k
+    (up to 64) alternatives, equal ones by the lower id; 32-bit arithmetic whatever the logits' type.
+
+    logits [rows, V] bf16, f16 or f32 with unit column stride; targets [rows] int64. A negative target (no
+    token there) gives 0, one of V or more gives NaN and raises bit 2 of `device_status`. -inf logits are
+    tokens of probability 0; a row of nothing else gives -inf and entropy 0; NaN and +inf give NaN."""
+    if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in _DT:
+        raise RuntimeError("logits must be a 2-D bf16, f16 or f32 CUDA tensor")
+    rows, V = logits.shape
+    if logits.numel() and ((V > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < V)):
+        raise RuntimeError("logits need unit column stride and rows that do not overlap")
+    if targets.dtype != torch.int64 or targets.shape != (rows,) or targets.device != logits.device or \
+            not targets.is_contiguous():
+        raise RuntimeError(f"targets must be a contiguous int64 tensor [{rows}] on {logits.device}")
+    if not 0 <= top_k <= min(64, V):
+        raise RuntimeError("need 0 <= top_k <= 64 and top_k <= V")
+    _no_grad_inputs(logits)
+    dev = logits.device
+    with torch.cuda.device(dev):
+        stats = torch.empty((2, rows), dtype=torch.float32, device=dev)
+        top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+        ids = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
+        rc = _lib.load().dscq_token_logprobs(logits.data_ptr(), _DT[logits.dtype], rows, V,
+                                             logits.stride(0) if rows > 1 else V, targets.data_ptr(), top_k,
+                                             stats[0].data_ptr(), stats[1].data_ptr(), top.data_ptr(),
+                                             ids.data_ptr(), _stream(dev))
+    _lib.check(rc, "token_logprobs")
+    return TokenLogprobs(stats[0], stats[1], top, ids)

@@ -56,7 +56,8 @@ int dscq_version(void);
 const char* dscq_last_error(void);
 
 /* Reads the sticky device status word of `device` (bit 0: a bounded wait in a
- * kernel expired; bit 1: bad launch geometry). Synchronises the device.
+ * kernel expired; bit 1: bad launch geometry; bit 2: a page, length, position or
+ * token id held in device memory was out of range and was left out). Synchronises the device.
  * `clear` != 0 resets it. */
 int dscq_device_status(int device, uint32_t* status, int clear);
 
@@ -239,6 +240,70 @@ int dscq_rowquant_tc_noalloc(const void* x, int x_dtype, int64_t M, int64_t K, i
 int dscq_rmsnorm(const void* x, const void* w, int64_t rows, int64_t H, float eps, void* y, void* stream);
 int dscq_rope(void* q, void* k, const void* cos_t, const void* sin_t, int64_t S, int Hq, int Hk, int D, void* stream);
 int dscq_silu_mul(const void* g, const void* u, int64_t n, void* y, void* stream);
+
+/*
+ * 4-bit paged key/value cache (no counterpart in the reference). One cached row is one token's D keys or
+ * values of one key head: D/2 bytes of codes 0..15 (element 2j in the low nibble of byte j) and two 16-bit
+ * numbers (step, low) of the cache's type; element = code * step + low.
+ *   codes  [pages, kv_heads, page_size, head_dim / 2] u8
+ *   affine [pages, kv_heads, page_size, 2] of `dtype` (DSCQ_BF16 or DSCQ_F16)
+ * A batch of sequences: rows q_start[b] .. q_start[b+1]-1 of the token axis are the newest tokens of sequence
+ * b, whose lengths[b] cached tokens include them (row i of n stands at position lengths[b] - n + i);
+ * page_table[b * ld_table + i] is the page of positions i * page_size ... Entries behind a sequence's last
+ * page are not read. q_start must not decrease. Rows outside [q_start[0], q_start[seqs]) belong to no sequence.
+ * head_dim is 64 or 128, page_size a power of two from 16 to 1024. Codes, queries, keys, values, tables and
+ * outputs are 16-byte aligned; strides are in elements and multiples of 8, the head dimension has stride 1.
+ * What these arrays hold is checked on the device: a position before the first or behind max_pages pages, or a
+ * page id outside [0, pages), is left out and raises bit 2 of dscq_device_status.
+ */
+typedef struct {
+  void* k_codes;
+  void* k_affine;
+  void* v_codes;
+  void* v_affine;
+  int64_t pages;
+  int32_t kv_heads, page_size, head_dim, dtype;
+  const int32_t* page_table;
+  int64_t ld_table, max_pages;
+  const int32_t* q_start;
+  const int32_t* lengths;
+  int64_t seqs;
+} dscq_kv4_batch;
+
+/*
+ * Rotates q and k by position (rotate-half form: y = x cos + rot(x) sin, rot(x) = [-x[D/2:], x[:D/2]]),
+ * quantises k and v row by row and writes them to their slots in the cache:
+ *   low = round(min y), step = round((max y - low) / 15), code = clamp(rint((y - low) / step), 0, 15),
+ *   code 0 where step is 0; a row whose low or step is not finite stores NaN for both.
+ * q [T, q_heads, D], k and v [T, kv_heads, D] of the cache's type with token and head strides; cos / sin
+ * [table_rows, D] by position, of the cache's type or float32 (table_dtype DSCQ_F32). q_out [T, q_heads, D]
+ * contiguous: the rotated queries, zero for rows of no sequence. Two rows of one call must not share a slot.
+ */
+int dscq_kv4_append(const dscq_kv4_batch* batch, const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                    int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h,
+                    int64_t T, int q_heads, const void* cos_t, const void* sin_t, int table_dtype, int64_t table_rows,
+                    void* q_out, void* stream);
+
+/* The values the cache holds for the rows of the token axis: k_out, v_out [T, kv_heads, D] of the cache's
+ * type, contiguous; zero for rows of no sequence. */
+int dscq_kv4_read(const dscq_kv4_batch* batch, int64_t T, void* k_out, void* v_out, void* stream);
+
+/*
+ * Causal attention of the rows of the token axis over the cache: out [T, q_heads, D] (contiguous) =
+ * softmax(scale * q k^T) v over the positions up to the row's own, query head h reading key head
+ * h / (q_heads / kv_heads). Rows of no sequence, and rows that see no key, are zero.
+ */
+int dscq_kv4_attention(const dscq_kv4_batch* batch, const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t T,
+                       int q_heads, float scale, void* out, void* stream);
+
+/*
+ * Log probability of targets[r], entropy and the k largest log probabilities of each row of logits
+ * [rows, V] (x_dtype, row stride ld elements): logprobs, entropy [rows] f32, top_logprobs [rows, k] f32 and
+ * top_ids [rows, k] i64, larger first and equal ones by the lower id (k = 0: both may be NULL; k <= 64 and
+ * k <= V). A negative target gives 0; one of V or more gives NaN and raises bit 2 of dscq_device_status.
+ */
+int dscq_token_logprobs(const void* logits, int x_dtype, int64_t rows, int64_t V, int64_t ld, const int64_t* targets,
+                        int k, float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids, void* stream);
 
 /* pack_int4, core/quantization.py:31-40. codes [rows, K] int8 (row stride
  * ld_codes) -> packed [rows, ceil(K/2)] (row stride ld_packed). Codes outside
