@@ -64,7 +64,8 @@ SIGNATURES = {
     "dscq_kv4_append": (_i32, [_kv4p, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _i32,
                                _i64, _vp, _vp]),
     "dscq_kv4_read": (_i32, [_kv4p, _i64, _vp, _vp, _vp]),
-    "dscq_kv4_attention": (_i32, [_kv4p, _vp, _i64, _i64, _i64, _i32, _f32, _vp, _vp]),
+    "dscq_kv4_attention_workspace": (_i64, [_i32]),
+    "dscq_kv4_attention": (_i32, [_kv4p, _vp, _i64, _i64, _i64, _i32, _i64, _f32, _vp, _vp, _i64, _vp]),
     "dscq_token_logprobs": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _vp]),
     "dscq_pack_int4": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "dscq_unpack_int4": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp]),

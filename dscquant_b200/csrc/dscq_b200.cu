@@ -7,6 +7,7 @@
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <limits>
 #include <map>
 #include <mutex>
 #include <string>
@@ -29,6 +30,7 @@
 #include "scatter_block.cuh"
 #include "kv4.cuh"
 #include "kv4_attention.cuh"
+#include "kv4_decode.cuh"
 #include "token_logprobs.cuh"
 
 namespace {
@@ -493,6 +495,8 @@ int kv4_batch(const dscq_kv4_batch* b, int64_t T, dscq::Kv4Batch* out) {
   return DSCQ_OK;
 }
 
+constexpr int kKv4Warps = 8, kKv4Stages = 2, kKv4Tile = 64;
+
 bool rows_ok(const void* p, int64_t st, int64_t sh) { return p && aligned(p, 16) && st % 8 == 0 && sh % 8 == 0; }
 
 template <typename T, int D>
@@ -514,11 +518,26 @@ cudaError_t launch_kv4_read(const dscq::Kv4Batch& b, int64_t rows, void* k, void
   return cudaGetLastError();
 }
 
-template <typename T, int D>
-cudaError_t launch_kv4_attention(const dscq::Kv4AttnParams& p, cudaStream_t st) {
-  const int64_t items = static_cast<int64_t>(p.T) * p.hq;
-  dscq::kv4_attention_rows<T, D><<<static_cast<unsigned>((items + 3) / 4), 128, 0, st>>>(p);
+template <typename T, int D, int NT>
+cudaError_t launch_kv4_decode(const dscq::Kv4AttnParams& a, int64_t max_rows, void* ws, cudaStream_t st) {
+  using C = dscq::Kv4DecodeConfig<D, NT, kKv4Warps, kKv4Stages, kKv4Tile>;
+  const int parts = num_sms();
+  dscq::Kv4DecodeParams p{a, max_rows, static_cast<float*>(ws), nullptr};
+  p.desc = reinterpret_cast<int*>(p.ws + static_cast<int64_t>(parts) * 2 * C::RB * (D + 2));
+  cudaError_t e = cudaFuncSetAttribute(dscq::kv4_decode_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       C::kSmem);
+  if (e != cudaSuccess) return e;
+  dscq::kv4_decode_kernel<T, C><<<parts, C::WARPS * 32, C::kSmem, st>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  dscq::kv4_decode_join<T, D, C::RB, C::TILE><<<parts, 256, 0, st>>>(p, parts);
   return cudaGetLastError();
+}
+
+template <typename T, int D>
+cudaError_t launch_kv4_attention(const dscq::Kv4AttnParams& a, int64_t max_q, void* ws, cudaStream_t st) {
+  const int64_t all = std::numeric_limits<int64_t>::max();
+  return max_q * a.group <= 8 ? launch_kv4_decode<T, D, 1>(a, all, ws, st) : launch_kv4_decode<T, D, 2>(a, all, ws, st);
 }
 
 // f.template operator()<T, D>() for the cache's type and head dimension.
@@ -1169,23 +1188,32 @@ int dscq_kv4_read(const dscq_kv4_batch* batch, int64_t T, void* k_out, void* v_o
   return DSCQ_OK;
 }
 
+int64_t dscq_kv4_attention_workspace(int head_dim) {
+  return head_dim == 64 || head_dim == 128 ? num_sms() * (2 * 16 * (head_dim + 2) * 4ll + 32) : 0;
+}
+
 int dscq_kv4_attention(const dscq_kv4_batch* batch, const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t T,
-                       int q_heads, float scale, void* out, void* stream) {
+                       int q_heads, int64_t max_q, float scale, void* out, void* workspace, int64_t workspace_bytes,
+                       void* stream) {
   dscq::Kv4AttnParams p{};
   int st = kv4_batch(batch, T, &p.b);
   if (st) return st;
   DSCQ_REQUIRE(q_heads >= 1 && q_heads <= 65536 && q_heads % batch->kv_heads == 0,
                "q_heads must be a multiple of kv_heads");
   DSCQ_REQUIRE(std::isfinite(scale), "scale must be finite");
+  DSCQ_REQUIRE(max_q >= 0, "max_q must not be negative");
   if (T == 0) return DSCQ_OK;
   DSCQ_REQUIRE(rows_ok(q, q_stride_t, q_stride_h) && out && aligned(out, 16),
                "q and out must be 16-byte aligned with strides that are multiples of 8");
+  DSCQ_REQUIRE(workspace && aligned(workspace, 16), "workspace must be 16-byte aligned");
   st = check_device(nullptr);
   if (st) return st;
+  DSCQ_REQUIRE(workspace_bytes >= dscq_kv4_attention_workspace(batch->head_dim),
+               "workspace is smaller than dscq_kv4_attention_workspace says");
   p.q = q, p.out = out, p.q_t = q_stride_t, p.q_h = q_stride_h;
   p.T = static_cast<int>(T), p.hq = q_heads, p.group = q_heads / batch->kv_heads;
   p.scale_log2 = scale * 1.4426950408889634f;
-#define DSCQ_CALL(TY, D) launch_kv4_attention<TY, D>(p, static_cast<cudaStream_t>(stream))
+#define DSCQ_CALL(TY, D) launch_kv4_attention<TY, D>(p, max_q ? std::min(max_q, T) : T, workspace, static_cast<cudaStream_t>(stream))
   cudaError_t e = DSCQ_KV4_DISPATCH(batch, DSCQ_CALL);
 #undef DSCQ_CALL
   if (e != cudaSuccess) return cuda_fail(e, "launch kv4_attention");

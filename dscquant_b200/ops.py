@@ -502,12 +502,16 @@ def kv4_attention(cache: PagedKV4, q: torch.Tensor, page_table: torch.Tensor, q_
     _no_grad_inputs(q)
     if q.shape[1] % cache.kv_heads or q.shape[1] == 0:
         raise RuntimeError("q's heads must be a multiple of the cache's")
+    if max_q is not None and max_q < 0:
+        raise RuntimeError("max_q must not be negative")
     batch = _kv4_batch(cache, page_table, q_start, lengths)
     with torch.cuda.device(dev):
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        rc = _lib.load().dscq_kv4_attention(batch, q.data_ptr(), q.stride(0), q.stride(1), T, q.shape[1],
-                                            cache.head_dim ** -0.5 if scale is None else float(scale),
-                                            out.data_ptr(), _stream(dev))
+        lib = _lib.load()
+        space = torch.empty(lib.dscq_kv4_attention_workspace(cache.head_dim), dtype=torch.uint8, device=dev)
+        rc = lib.dscq_kv4_attention(batch, q.data_ptr(), q.stride(0), q.stride(1), T, q.shape[1], max_q or 0,
+                                    cache.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(),
+                                    space.data_ptr(), space.numel(), _stream(dev))
     _lib.check(rc, "kv4_attention")
     return out
 

@@ -288,13 +288,19 @@ int dscq_kv4_append(const dscq_kv4_batch* batch, const void* q, int64_t q_stride
  * type, contiguous; zero for rows of no sequence. */
 int dscq_kv4_read(const dscq_kv4_batch* batch, int64_t T, void* k_out, void* v_out, void* stream);
 
+/* Bytes of workspace dscq_kv4_attention needs on the current device (0: unsupported head_dim). */
+int64_t dscq_kv4_attention_workspace(int head_dim);
+
 /*
  * Causal attention of the rows of the token axis over the cache: out [T, q_heads, D] (contiguous) =
  * softmax(scale * q k^T) v over the positions up to the row's own, query head h reading key head
- * h / (q_heads / kv_heads). Rows of no sequence, and rows that see no key, are zero.
+ * h / (q_heads / kv_heads). Rows of no sequence, and rows that see no key, are zero. `max_q` is the most rows
+ * any sequence has in this call (0: unknown); it decides which kernels run. `workspace` (16-byte aligned) is
+ * scratch of this call until it has run: calls that may overlap on the GPU need one each.
  */
 int dscq_kv4_attention(const dscq_kv4_batch* batch, const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t T,
-                       int q_heads, float scale, void* out, void* stream);
+                       int q_heads, int64_t max_q, float scale, void* out, void* workspace, int64_t workspace_bytes,
+                       void* stream);
 
 /*
  * Log probability of targets[r], entropy and the k largest log probabilities of each row of logits

@@ -34,7 +34,7 @@ def test_batch_refusals(native, buf, changes, word):
     b = batch(buf, **changes)
     for rc in (native.dscq_kv4_append(b, buf, 256, 128, buf, 256, 128, buf, 256, 128, 1, 2, buf, buf, 0, 10, buf, None),
                native.dscq_kv4_read(b, 1, buf, buf, None),
-               native.dscq_kv4_attention(b, buf, 256, 128, 1, 2, 1.0, buf, None)):
+               native.dscq_kv4_attention(b, buf, 256, 128, 1, 2, 1, 1.0, buf, buf, 1 << 30, None)):
         assert rc == _lib.DSCQ_ERR_INVALID and word in _lib.last_error()
 
 
@@ -66,12 +66,14 @@ def test_attention_refusals(native, buf):
     from dscquant_b200 import _lib
 
     b = batch(buf)
-    for args, word in (((buf, 256, 128, 1, 3, 1.0, buf), "multiple of kv_heads"), ((buf, 256, 128, 1, 0, 1.0, buf), "q_heads"),
-                       ((buf, 256, 128, 1, 2, float("nan"), buf), "scale"), ((buf, 256, 128, 1, 2, float("inf"), buf), "scale"),
-                       ((None, 256, 128, 1, 2, 1.0, buf), "q and out"), ((buf, 250, 128, 1, 2, 1.0, buf), "multiples"),
-                       ((buf, 256, 128, 1, 2, 1.0, buf + 8), "aligned")):
-        assert native.dscq_kv4_attention(b, *args, None) == _lib.DSCQ_ERR_INVALID
-        assert word in _lib.last_error(), args
+    good = dict(q=buf, qt=256, qh=128, T=1, hq=2, max_q=1, scale=1.0, out=buf, ws=buf, bytes=1 << 30)
+    for change, word in ((dict(hq=3), "multiple of kv_heads"), (dict(hq=0), "q_heads"), (dict(scale=float("nan")), "scale"),
+                         (dict(scale=float("inf")), "scale"), (dict(q=None), "q and out"), (dict(qt=250), "multiples"),
+                         (dict(out=buf + 8), "aligned"), (dict(max_q=-1), "max_q"), (dict(ws=None), "workspace"),
+                         (dict(ws=buf + 4), "workspace")):
+        rc = native.dscq_kv4_attention(b, *{**good, **change}.values(), None)
+        assert rc == _lib.DSCQ_ERR_INVALID and word in _lib.last_error(), change
+    assert native.dscq_kv4_attention(b, *{**good, "T": 0}.values(), None) == _lib.DSCQ_OK
 
 
 def test_logprob_refusals(native, buf):
@@ -95,7 +97,7 @@ def test_valid_calls_without_gpu_fail_cleanly(native, buf):
     b = batch(buf)
     failed = (_lib.DSCQ_ERR_CUDA, _lib.DSCQ_ERR_UNSUPPORTED)
     assert native.dscq_kv4_read(b, 1, buf, buf, None) in failed
-    assert native.dscq_kv4_attention(b, buf, 256, 128, 1, 2, 1.0, buf, None) in failed
+    assert native.dscq_kv4_attention(b, buf, 256, 128, 1, 2, 1, 1.0, buf, buf, 1 << 30, None) in failed
     assert native.dscq_token_logprobs(buf, 0, 1, 10, 10, buf, 0, buf, buf, None, None, None) in failed
 
 
