@@ -495,8 +495,6 @@ int kv4_batch(const dscq_kv4_batch* b, int64_t T, dscq::Kv4Batch* out) {
   return DSCQ_OK;
 }
 
-constexpr int kKv4Warps = 8, kKv4Stages = 2, kKv4Tile = 64;
-
 bool rows_ok(const void* p, int64_t st, int64_t sh) { return p && aligned(p, 16) && st % 8 == 0 && sh % 8 == 0; }
 
 template <typename T, int D>
@@ -518,20 +516,33 @@ cudaError_t launch_kv4_read(const dscq::Kv4Batch& b, int64_t rows, void* k, void
   return cudaGetLastError();
 }
 
+template <int D, int NT>
+using Kv4Decode = dscq::Kv4DecodeConfig<D, NT, NT == 1 ? 12 : 8, 2, 64>;
+
 template <typename T, int D, int NT>
 cudaError_t launch_kv4_decode(const dscq::Kv4AttnParams& a, int64_t max_rows, void* ws, cudaStream_t st) {
-  using C = dscq::Kv4DecodeConfig<D, NT, kKv4Warps, kKv4Stages, kKv4Tile>;
+  using C = Kv4Decode<D, NT>;
   const int parts = num_sms();
-  dscq::Kv4DecodeParams p{a, max_rows, static_cast<float*>(ws), nullptr};
-  p.desc = reinterpret_cast<int*>(p.ws + static_cast<int64_t>(parts) * 2 * C::RB * (D + 2));
+  dscq::Kv4DecodeParams p{a, max_rows, static_cast<float*>(ws), nullptr, nullptr};
+  p.warp = p.cta + static_cast<int64_t>(parts) * 2 * C::kPiece;
+  p.desc = reinterpret_cast<int*>(p.warp + static_cast<int64_t>(parts) * C::WARPS * C::kPiece);
   cudaError_t e = cudaFuncSetAttribute(dscq::kv4_decode_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        C::kSmem);
   if (e != cudaSuccess) return e;
   dscq::kv4_decode_kernel<T, C><<<parts, C::WARPS * 32, C::kSmem, st>>>(p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  dscq::kv4_decode_join<T, D, C::RB, C::TILE><<<parts, 256, 0, st>>>(p, parts);
-  return cudaGetLastError();
+  // launched while the first kernel still runs; waits for its results on the device
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(parts);
+  cfg.blockDim = dim3(8 * C::RB);
+  cfg.stream = st;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, dscq::kv4_decode_join<T, D, C::RB, C::TILE>, p, parts);
 }
 
 template <typename T, int D>
@@ -1189,7 +1200,9 @@ int dscq_kv4_read(const dscq_kv4_batch* batch, int64_t T, void* k_out, void* v_o
 }
 
 int64_t dscq_kv4_attention_workspace(int head_dim) {
-  return head_dim == 64 || head_dim == 128 ? num_sms() * (2 * 16 * (head_dim + 2) * 4ll + 32) : 0;
+  if (head_dim == 64) return std::max(Kv4Decode<64, 1>::workspace(num_sms()), Kv4Decode<64, 2>::workspace(num_sms()));
+  if (head_dim == 128) return std::max(Kv4Decode<128, 1>::workspace(num_sms()), Kv4Decode<128, 2>::workspace(num_sms()));
+  return 0;
 }
 
 int dscq_kv4_attention(const dscq_kv4_batch* batch, const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t T,
@@ -1211,7 +1224,8 @@ int dscq_kv4_attention(const dscq_kv4_batch* batch, const void* q, int64_t q_str
   DSCQ_REQUIRE(workspace_bytes >= dscq_kv4_attention_workspace(batch->head_dim),
                "workspace is smaller than dscq_kv4_attention_workspace says");
   p.q = q, p.out = out, p.q_t = q_stride_t, p.q_h = q_stride_h;
-  p.T = static_cast<int>(T), p.hq = q_heads, p.group = q_heads / batch->kv_heads;
+  p.T = static_cast<int>(T), p.hq = q_heads;
+  p.set_group(q_heads / batch->kv_heads);
   p.scale_log2 = scale * 1.4426950408889634f;
 #define DSCQ_CALL(TY, D) launch_kv4_attention<TY, D>(p, max_q ? std::min(max_q, T) : T, workspace, static_cast<cudaStream_t>(stream))
   cudaError_t e = DSCQ_KV4_DISPATCH(batch, DSCQ_CALL);

@@ -12,7 +12,20 @@ struct Kv4AttnParams {
   void* out;  // [T, hq, D] contiguous
   int64_t q_t, q_h;
   int T, hq, group;
-  float scale_log2;  // scale * log2(e)
+  uint32_t group_mul, group_shift;  // r / group by multiplication (row_token)
+  float scale_log2;                 // scale * log2(e)
+
+  void set_group(int g) {
+    group = g;
+    group_shift = 0;
+    while ((1u << group_shift) < static_cast<uint32_t>(g)) ++group_shift;
+    group_mul = static_cast<uint32_t>(((uint64_t(1) << 32) * ((uint64_t(1) << group_shift) - g)) / g + 1);
+  }
+  // r / group for 0 <= r < 2^31: (r + floor(r m / 2^32)) >> shift with m = 2^32 (2^shift - group) / group + 1.
+  __device__ __forceinline__ int row_token(int r) const {
+    const uint32_t u = static_cast<uint32_t>(r);
+    return static_cast<int>((__umulhi(u, group_mul) + u) >> group_shift);
+  }
 };
 
 }  // namespace dscq

@@ -1,13 +1,14 @@
 // Attention of few rows per sequence (single tokens, drafts) over the 4-bit paged cache: bound by reading the
 // cache once. See kv4_attention.cuh for the operator.
 //
-// Mathematics. With n the 4-bit code, (step, low) of a row and c' = 1 + n/16 (one shift and one LOP3 put two
-// codes into the mantissas of two 16-bit numbers, exactly):
-//   q.k = 16 step (q.c') + (low - 16 step) sum(q)          -- q.c' on the tensor cores, the rest per key
-//   o   = 16/F (sum_t P'_t c'_t - sum_t P'_t) + sum_t p_t low_t,   P'_t = round16(F p_t step_t)
-// so no element is ever dequantised; step and low cost a few operations per key, not per element. Scores,
-// softmax statistics and sums are 32-bit; only the weights P' are rounded to 16 bits, as the tensor cores
-// take them (F = 16 for bf16; 4 for f16, whose range F step must not leave).
+// Mathematics. A 4-bit code n in the low bits of an fp16 number is the subnormal n 2^-24 (n 2^-20 four bits up), which
+// tensor cores multiply exactly; so an AND (and one shift for every other pair) makes two operands of two codes:
+//   q.k = step (q.n) + low sum(q)
+//   o   = sum_t P'_t n_t / F + sum_t p_t low_t,   P'_t = fp16(F p_t step_t)
+// No element is ever dequantised; step and low cost a few operations per key, not per element. Queries
+// enter as fp16, each row scaled by a power of two to the top of its range (exact but for elements 2^-29 below
+// the row's largest); F is a power of two that follows the largest step seen, so P' stays in range for any
+// step. Scores, softmax statistics and sums are 32-bit; only the weights P' are rounded, to 11 bits.
 //
 // Fragments (mma.m16n8k16). Scores: A = 16 keys x 16 dims, B = 8 query rows; a lane's 32 dims (16 for D = 64)
 // of a key are one 16-byte load, any dim order works as long as the queries use the same. Output: A = 16
@@ -27,42 +28,22 @@ namespace dscq {
 struct Kv4DecodeParams {
   Kv4AttnParams a;
   int64_t max_rows;  // sequences with more rows * group than this are not this kernel's
-  float* ws;         // [G][2][8 NT][D + 2]: rows' sums, then their maxima and weights' sums
+  // A piece of a cut run is [8 NT][D] sums of its rows, then their maxima and weights' sums (32-bit).
+  float* cta;        // [G][2] pieces of runs cut by CTA borders
+  float* warp;       // [G][WARPS] pieces of runs cut at a warp's start
   int* desc;         // [G][8]: slot 0 {valid, ends}, slot 1 {valid, b, h, block}
 };
 
-template <typename T>
-struct Kv4Mma;
-template <>
-struct Kv4Mma<__nv_bfloat16> {
-  static constexpr uint32_t kOne = 0x3F803F80u, kMask = 0x00780078u;
-  static constexpr int kShift = 3;  // code's place in the mantissa
-  static constexpr float kF = 16.f;
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-};
-template <>
-struct Kv4Mma<__half> {
-  static constexpr uint32_t kOne = 0x3C003C00u, kMask = 0x03C003C0u;
-  static constexpr int kShift = 6;
-  static constexpr float kF = 4.f;
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-};
-
-// Codes I and I + 4 of `w` as the pair (1 + n/16, 1 + n'/16).
-template <typename T, int I>
-__device__ __forceinline__ uint32_t kv4_pair(uint32_t w) {
-  constexpr int s = Kv4Mma<T>::kShift - 4 * I;
-  const uint32_t x = s >= 0 ? w << (s >= 0 ? s : 0) : w >> (s < 0 ? -s : 0);
-  return (x & Kv4Mma<T>::kMask) | Kv4Mma<T>::kOne;
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+
+// 2^e as a float, -126 <= e <= 127.
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+// floor(log2 x) of a positive normal x.
+__device__ __forceinline__ int log2i(float x) { return static_cast<int>(__float_as_uint(x) >> 23) - 127; }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -74,6 +55,8 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+
+constexpr uint32_t kCode0 = 0x000F000Fu, kCode1 = 0x00F000F0u;  // two codes of a word: weights 2^-24 and 2^-20
 
 // One sequence as the decode kernel sees it.
 struct Kv4Seq {
@@ -97,6 +80,72 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttnParams& a, int64_t max_ro
   return r;
 }
 
+// Four rows of a run being put together from its pieces, by one warp: lane's dims are D/32 from lane * D/32.
+template <int D>
+struct Kv4Joined {
+  static constexpr int E = D / 32;
+  float m[4], l[4], y[4][E];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[r][e] = 0.f;
+    }
+  }
+  __device__ __forceinline__ void add(const float* piece, int RB, int row0, int lane) {
+    const float4 pm = *reinterpret_cast<const float4*>(piece + RB * D + row0);
+    const float4 pl = *reinterpret_cast<const float4*>(piece + RB * D + RB + row0);
+    const float ms[4] = {pm.x, pm.y, pm.z, pm.w}, ls[4] = {pl.x, pl.y, pl.z, pl.w};
+    float x[4][E];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float* src = piece + (row0 + r) * D + lane * E;
+      if constexpr (E == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(src);
+        x[r][0] = v.x, x[r][1] = v.y, x[r][2] = v.z, x[r][3] = v.w;
+      } else {
+        const float2 v = *reinterpret_cast<const float2*>(src);
+        x[r][0] = v.x, x[r][1] = v.y;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float n = fmaxf(m[r], ms[r]), nb = n == -INFINITY ? 0.f : n;
+      const float f = ex2(m[r] - nb), g = ex2(ms[r] - nb);
+      m[r] = n;
+      l[r] = fmaf(l[r], f, ls[r] * g);
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[r][e] = fmaf(y[r][e], f, x[r][e] * g);
+    }
+  }
+  __device__ __forceinline__ void store(float* piece, int RB, int row0, int lane) const {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) piece[(row0 + r) * D + lane * E + e] = y[r][e];
+      if (lane == r) {
+        piece[RB * D + row0 + r] = m[r];
+        piece[RB * D + RB + row0 + r] = l[r];
+      }
+    }
+  }
+  // Rows rr .. rr + 3 of sequence sq and key head h.
+  template <typename T>
+  __device__ __forceinline__ void write(const Kv4AttnParams& a, const Kv4Seq& sq, int h, int rr, int lane) const {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (rr + r >= sq.n * a.group) break;
+      T* out = static_cast<T*>(a.out) + ((sq.q0 + static_cast<int64_t>(a.row_token(rr + r))) * a.hq + h * a.group +
+                                         rr + r - a.row_token(rr + r) * a.group) * D + lane * E;
+      const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+#pragma unroll
+      for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(out + e) = pack2<T>(y[r][e] * inv, y[r][e + 1] * inv);
+    }
+  }
+};
+
 template <int D_, int NT_, int WARPS_, int STAGES_, int TILE_>
 struct Kv4DecodeConfig {
   static constexpr int D = D_, NT = NT_, WARPS = WARPS_, STAGES = STAGES_, TILE = TILE_;
@@ -104,25 +153,25 @@ struct Kv4DecodeConfig {
   static constexpr int kCodes = TILE * D / 2;             // bytes of one side's codes in a stage
   static constexpr int kStage = 2 * kCodes + 2 * TILE * 4;
   static constexpr int kRing = STAGES * kStage;
-  static constexpr int kPiece = RB * (D + 2) * 4;         // a cut run's piece
-  static constexpr int kSmem = WARPS * (kRing + kPiece) + WARPS * STAGES * 12 + 1024;
-  static_assert(kRing >= kPiece, "the last piece of a warp goes into its ring");
-  static_assert(2 * WARPS <= 32 && kStage % 16 == 0 && kPiece % 16 == 0, "layout");
+  static constexpr int kPiece = RB * (D + 2);             // floats of a cut run's piece
+  static constexpr int kSmem = WARPS * kRing + WARPS * STAGES * 12;
+  static constexpr int64_t workspace(int64_t parts) { return parts * ((2 + WARPS) * kPiece * 4 + 32); }
+  static_assert(kRing >= kPiece * 4, "the last piece of a warp goes into its ring");
+  static_assert(2 * WARPS <= 32 && kStage % 16 == 0 && kPiece % 4 == 0, "layout");
 };
 
 template <typename T, class C>
 __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4DecodeParams p) {
-  using M = Kv4Mma<T>;
   constexpr int D = C::D, NT = C::NT, TILE = C::TILE, WARPS = C::WARPS, STAGES = C::STAGES, RB = C::RB;
   constexpr int KB = TILE / 16;  // 16-key blocks of a tile
   constexpr int W4 = D / 32;     // words of codes a lane takes of a key
   const Kv4AttnParams& a = p.a;
   extern __shared__ __align__(128) uint8_t kv4_smem[];
-  uint8_t* first_all = kv4_smem + WARPS * C::kRing;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(first_all + WARPS * C::kPiece);
+  float* first_all = p.warp + blockIdx.x * static_cast<int64_t>(WARPS * C::kPiece);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(kv4_smem + WARPS * C::kRing);
   uint32_t* vmask_all = reinterpret_cast<uint32_t*>(bars + WARPS * STAGES);
-  __shared__ int64_t scan[WARPS + 1];
-  __shared__ int where[WARPS][4];    // sequence, head, block, tile a warp starts at
+  __shared__ int64_t scan[WARPS];
+  __shared__ int64_t tiles_before[WARPS * 32];  // of each thread's sequences
   __shared__ int piece[2 * WARPS][6];  // valid, starts, ends, b, h, block; pieces 2w (cut at its start), 2w + 1
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
@@ -170,40 +219,63 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
     total += scan[w];
   }
   before += incl - mine;
-  // a warp has at least one tile where there are enough; CTAs beyond that have none
-  const int64_t parts = max(min(total / WARPS, static_cast<int64_t>(gridDim.x)), static_cast<int64_t>(1));
-  const int64_t shares = parts * WARPS;
-  for (int w = 0; w < WARPS; ++w) {
-    const int64_t at = total * (static_cast<int64_t>(blockIdx.x) * WARPS + w) / shares;
-    if (at >= before && at < before + mine) {
-      int64_t left = at - before;
-      for (int s = s_lo; s < s_hi; ++s) {
-        const Kv4Seq r = kv4_seq<TILE, RB>(a, p.max_rows, s);
-        const int64_t units = static_cast<int64_t>(r.blocks) * r.tiles * a.b.hk;
-        if (left < units) {
-          const int64_t run = left / r.tiles;
-          where[w][0] = s;
-          where[w][1] = static_cast<int>(run / r.blocks);
-          where[w][2] = static_cast<int>(run % r.blocks);
-          where[w][3] = static_cast<int>(left % r.tiles);
-          break;
-        }
-        left -= units;
-      }
-    }
-  }
+  tiles_before[tid] = before;
+  // Equal shares: warp g of the launch begins at tile g * base + min(g, extra). A warp has at least one tile
+  // where there are enough; CTAs beyond that have none.
+  const int parts = static_cast<int>(max(min(total / WARPS, static_cast<int64_t>(gridDim.x)), static_cast<int64_t>(1)));
+  const int shares = parts * WARPS;
+  const int64_t base = total >> 32 ? total / shares : static_cast<uint32_t>(total) / static_cast<uint32_t>(shares);
+  const int extra = static_cast<int>(total - base * shares);
+  const int gw = blockIdx.x * WARPS + warp;
+  const int count = gw < shares ? static_cast<int>(base) + (gw < extra) : 0;
   __syncthreads();
-
-  const int64_t gw = static_cast<int64_t>(blockIdx.x) * WARPS + warp;
-  const int64_t count = gw < shares ? total * (gw + 1) / shares - total * gw / shares : 0;
   struct Cursor {
     int b, h, blk, t;
     Kv4Seq s;
   };
-  Cursor c{where[warp][0], where[warp][1], where[warp][2], where[warp][3], {}};
-  if (count > 0) c.s = kv4_seq<TILE, RB>(a, p.max_rows, c.b);
+  Cursor c{};
+  if (count > 0) {
+    // The thread whose sequences hold the warp's first tile, then the sequence among them.
+    int64_t left = gw * base + min(gw, extra);
+    unsigned le = __ballot_sync(0xffffffffu, tiles_before[lane * WARPS] <= left);
+    int th = (31 - __clz(le)) * WARPS;
+    le = __ballot_sync(0xffffffffu, lane < WARPS && tiles_before[th + (lane < WARPS ? lane : 0)] <= left);
+    th += 31 - __clz(le);
+    left -= tiles_before[th];
+    for (int s0 = th * per;; s0 += 32) {
+      const int s = s0 + lane;
+      Kv4Seq r{};
+      if (s < min(th * per + per, B)) r = kv4_seq<TILE, RB>(a, p.max_rows, s);
+      const int64_t units = static_cast<int64_t>(r.blocks) * r.tiles * a.b.hk;
+      int64_t upto = units;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, upto > left);
+      if (!past && s0 + 32 < min(th * per + per, B)) {
+        left -= __shfl_sync(0xffffffffu, upto, 31);
+        continue;
+      }
+      const int src = past ? __ffs(past) - 1 : 31;
+      left -= __shfl_sync(0xffffffffu, upto - units, src);
+      c.b = s0 + src;
+      c.s.q0 = __shfl_sync(0xffffffffu, r.q0, src);
+      c.s.n = __shfl_sync(0xffffffffu, r.n, src);
+      c.s.len = __shfl_sync(0xffffffffu, r.len, src);
+      c.s.tiles = max(__shfl_sync(0xffffffffu, r.tiles, src), 1);
+      c.s.blocks = max(__shfl_sync(0xffffffffu, r.blocks, src), 1);
+      c.s.keys = __shfl_sync(0xffffffffu, r.keys, src);
+      break;
+    }
+    const int64_t run = left >> 32 ? left / c.s.tiles : static_cast<uint32_t>(left) / static_cast<uint32_t>(c.s.tiles);
+    c.t = static_cast<int>(left - run * c.s.tiles);
+    c.h = static_cast<int>(run >> 32 ? run / c.s.blocks : static_cast<uint32_t>(run) / static_cast<uint32_t>(c.s.blocks));
+    c.blk = static_cast<int>(run - static_cast<int64_t>(c.h) * c.s.blocks);
+  }
   Cursor pr = c;  // the tile to fetch next
-  auto advance = [&](Cursor& x, bool more) {
+  auto advance = [&](Cursor& x, bool more) {  // more: there is a tile behind this one
     if (++x.t < x.s.tiles) return;
     x.t = 0;
     if (++x.blk < x.s.blocks) return;
@@ -216,22 +288,28 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
   };
   const int pl2 = min(a.b.ps_log2, TILE == 64 ? 6 : TILE == 32 ? 5 : 4);  // log2 of the keys one copy brings
   const int pieces = TILE >> pl2;
-  // Fetches tile `pr` into `stage`: lane i < pieces copies the i-th run of keys that lie in one page.
-  auto fetch = [&](int stage) {
+  // Lane i < pieces brings the i-th run of a tile's keys that lies in one page. The page of the next tile is
+  // looked up while the current one is worked on.
+  int page = -1;
+  bool want = false;
+  auto look = [&] {
     const int key = pr.t * TILE + (lane << pl2);
-    const bool want = lane < pieces && key < pr.s.keys;
-    int64_t page = -1;
-    if (want) page = a.b.table[pr.b * a.b.ld_table + (key >> a.b.ps_log2)];
+    want = lane < pieces && key < pr.s.keys;
+    page = want ? a.b.table[pr.b * a.b.ld_table + (key >> a.b.ps_log2)] : -1;
+  };
+  auto fetch = [&](int stage) {
     const bool ok = want && page >= 0 && page < a.b.pages;
-    const unsigned got = __ballot_sync(0xffffffffu, ok), wanted = __ballot_sync(0xffffffffu, want);
+    const unsigned got = __ballot_sync(0xffffffffu, ok);
+    const bool all = got == __ballot_sync(0xffffffffu, want);
     if (lane == 0) {
-      vmask[stage] = got | (got != wanted ? 0x80000000u : 0u);
-      if (got != wanted) raise_status(kStatusBadIndex);
+      vmask[stage] = got | (all ? 0u : 0x80000000u);
+      if (!all) raise_status(kStatusBadIndex);
       mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(__popc(got)) * (static_cast<uint32_t>(D + 8) << pl2));
     }
     __syncwarp();
     if (ok) {
-      const int64_t row = ((page * a.b.hk + pr.h) << a.b.ps_log2) + (key & ((1 << a.b.ps_log2) - 1));
+      const int in_page = (pr.t * TILE + (lane << pl2)) & ((1 << a.b.ps_log2) - 1);
+      const int64_t row = ((static_cast<int64_t>(page) * a.b.hk + pr.h) << a.b.ps_log2) + in_page;
       uint8_t* st = ring + stage * C::kStage;
       const uint32_t cb = static_cast<uint32_t>(D / 2) << pl2, ab = 4u << pl2;
       bulk_load_g2s(st + lane * cb, a.b.kc + row * (D / 2), cb, &full[stage]);
@@ -240,63 +318,89 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
       bulk_load_g2s(st + 2 * C::kCodes + TILE * 4 + lane * ab, a.b.va + row, ab, &full[stage]);
     }
   };
-  int64_t fetched = 0;
-  for (; fetched < STAGES && fetched < count; ++fetched) {
-    fetch(static_cast<int>(fetched));
-    advance(pr, fetched + 1 < count);
-  }
+  int fetched = 0;
+  if (count > 0) look();
+  auto fetch_next = [&](int stage) {
+    fetch(stage);
+    if (++fetched < count) {
+      advance(pr, true);
+      look();
+    }
+  };
+  while (fetched < STAGES && fetched < count) fetch_next(fetched);
 
-  float o[NT][D / 16][4], ones[NT][4], mx[NT][2], l[NT][2], low[NT][2], sumq[NT][2];
+  // mx is the running maximum of the scores in their rows' own units, c1 turns those into powers of two
+  float o[NT][D / 16][4], mx[NT][2], l[NT][2], low[NT][2], sumq[NT][2], c1[NT][2];
   uint32_t qf[NT][W4][4];
-  int lim[NT][2], min_lim = 0, t0 = 0;
+  int lim[NT][2], min_lim = 0, max_lim = 0, t0 = 0;
+  int vexp = 0;  // every step of the values so far is below 2^vexp
   bool failed = false;
   int stage = 0;
   uint32_t parity = 0;
-  for (int64_t i = 0; i < count; ++i) {
+  for (int i = 0; i < count; ++i) {
     const int rows = c.s.n * a.group;  // at most max_rows, or of a sequence whose rows fit 31 bits
     const int r0 = c.blk * RB;
     if (i == 0 || c.t == 0) {
       // ---- a run (or the rest of one) begins: its queries, in the lane order of the codes
       t0 = c.t;
       min_lim = INT_MAX;
+      max_lim = 0;
+      vexp = -100;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int r = r0 + nt * 8 + g;
-        float sum = 0.f;
-        const T* src = static_cast<const T*>(a.q) + (c.s.q0 + static_cast<int64_t>(r / a.group)) * a.q_t +
-                       (static_cast<int64_t>(c.h) * a.group + r % a.group) * a.q_h + q * (D / 4);
+        const int tok = a.row_token(r);
+        const T* src = static_cast<const T*>(a.q) + (c.s.q0 + static_cast<int64_t>(tok)) * a.q_t +
+                       (static_cast<int64_t>(c.h) * a.group + (r - tok * a.group)) * a.q_h + q * (D / 4);
+        float x[W4][8], sum = 0.f, big = 0.f;
 #pragma unroll
         for (int w = 0; w < W4; ++w) {
           uint4 v = make_uint4(0, 0, 0, 0);
           if (r < rows) v = *reinterpret_cast<const uint4*>(src + 8 * w);
-          const float2 f0 = unpack2<T>(v.x), f1 = unpack2<T>(v.y), f2 = unpack2<T>(v.z), f3 = unpack2<T>(v.w);
-          sum += ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
-          qf[nt][w][0] = __byte_perm(v.x, v.z, 0x5410);  // elements 0, 4
-          qf[nt][w][1] = __byte_perm(v.x, v.z, 0x7632);  // 1, 5
-          qf[nt][w][2] = __byte_perm(v.y, v.w, 0x5410);  // 2, 6
-          qf[nt][w][3] = __byte_perm(v.y, v.w, 0x7632);  // 3, 7
+          kv4_unpack8<T>(v, x[w]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            sum += x[w][e];
+            big = fmaxf(big, fabsf(x[w][e]));
+          }
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        // the row's largest element goes to [2^14, 2^15); a negative scale turns the queries around
+        const int k = big > 0.f && big < INFINITY ? min(max(14 - log2i(big), -90), 120) : 0;
+        const float qs = a.scale_log2 == 0.f ? 0.f : copysignf(pow2f(k), a.scale_log2);
+#pragma unroll
+        for (int w = 0; w < W4; ++w)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float f = e & 1 ? qs * 0.0625f : qs;  // codes four bits up count sixteenfold
+            qf[nt][w][e] = pack2<__half>(x[w][e] * f, x[w][e + 4] * f);
+          }
+        const float sq = sum * qs * 0x1p-24f, cc = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2) * pow2f(24 - k);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          sumq[nt][j] = __shfl_sync(0xffffffffu, sum, (2 * q + j) * 4);
+          sumq[nt][j] = __shfl_sync(0xffffffffu, sq, (2 * q + j) * 4);
+          c1[nt][j] = __shfl_sync(0xffffffffu, cc, (2 * q + j) * 4);
           const int rr = r0 + nt * 8 + 2 * q + j;
           // keys the row sees: positions up to its own
-          lim[nt][j] = rr < rows ? min(c.s.keys, c.s.len - c.s.n + rr / a.group + 1) : c.s.keys;
-          min_lim = min(min_lim, lim[nt][j]);
+          lim[nt][j] = rr < rows ? min(c.s.keys, c.s.len - c.s.n + a.row_token(rr) + 1) : 0;
+          min_lim = min(min_lim, rr < rows ? lim[nt][j] : c.s.keys);
+          max_lim = max(max_lim, lim[nt][j]);
           mx[nt][j] = -INFINITY;
           l[nt][j] = low[nt][j] = 0.f;
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) ones[nt][e] = 0.f;
 #pragma unroll
         for (int d = 0; d < D / 16; ++d)
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[nt][d][e] = 0.f;
       }
-      min_lim = min(min_lim, __shfl_xor_sync(0xffffffffu, min_lim, 1));
-      min_lim = min(min_lim, __shfl_xor_sync(0xffffffffu, min_lim, 2));
+#pragma unroll
+      for (int sh = 1; sh < 4; sh <<= 1) {
+        min_lim = min(min_lim, __shfl_xor_sync(0xffffffffu, min_lim, sh));
+        max_lim = max(max_lim, __shfl_xor_sync(0xffffffffu, max_lim, sh));
+      }
     }
 
     if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], parity, nullptr))) {
@@ -309,6 +413,29 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
     const uint32_t have = vmask[stage];
     const int key0 = c.t * TILE;
     const bool masked = key0 + TILE > min_lim || (have & 0x80000000u);
+
+    // ---- the values' steps: F follows the largest
+    uint32_t va[KB][2];
+    float vmax = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int at = 16 * kb + 8 * j + g;
+        va[kb][j] = vaff[at];
+        // what no row sees may hold anything
+        if (masked && (key0 + at >= max_lim || !((have >> (at >> pl2)) & 1u))) va[kb][j] = 0;
+        vmax = fmaxf(vmax, unpack2<T>(va[kb][j]).x);
+      }
+    float shrink = 1.f;
+    if (__any_sync(0xffffffffu, vmax >= pow2f(vexp))) {
+#pragma unroll
+      for (int sh = 4; sh < 32; sh <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, sh));
+      const int e = min(log2i(vmax) + 1, 127);
+      shrink = e - vexp > 126 ? 0.f : pow2f(vexp - e);
+      vexp = e;
+    }
+    const float vf = vexp < -99 ? 0.f : pow2f(min(14 - vexp, 127));
 
     // ---- scores of the tile: s[nt][kb][.]: keys 16 kb + g (0, 1) and + 8 (2, 3), rows 2q (0, 2) and 2q + 1
     float s[NT][KB][4];
@@ -331,23 +458,22 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
         for (int e = 0; e < 4; ++e) s[nt][kb][e] = 0.f;
 #pragma unroll
       for (int w = 0; w < W4; ++w) {
-        const uint32_t a0[4] = {kv4_pair<T, 0>(w0[w]), kv4_pair<T, 0>(w1[w]), kv4_pair<T, 1>(w0[w]), kv4_pair<T, 1>(w1[w])};
-        const uint32_t a1[4] = {kv4_pair<T, 2>(w0[w]), kv4_pair<T, 2>(w1[w]), kv4_pair<T, 3>(w0[w]), kv4_pair<T, 3>(w1[w])};
+        const uint32_t u0 = w0[w] >> 8, u1 = w1[w] >> 8;
+        const uint32_t a0[4] = {w0[w] & kCode0, w1[w] & kCode0, w0[w] & kCode1, w1[w] & kCode1};
+        const uint32_t a1[4] = {u0 & kCode0, u1 & kCode0, u0 & kCode1, u1 & kCode1};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          M::mma(s[nt][kb], a0, qf[nt][w][0], qf[nt][w][1]);
-          M::mma(s[nt][kb], a1, qf[nt][w][2], qf[nt][w][3]);
+          mma_f16(s[nt][kb], a0, qf[nt][w][0], qf[nt][w][1]);
+          mma_f16(s[nt][kb], a1, qf[nt][w][2], qf[nt][w][3]);
         }
       }
       const float2 k0 = unpack2<T>(kaff[16 * kb + g]), k1 = unpack2<T>(kaff[16 * kb + 8 + g]);
-      const float m0 = 16.f * a.scale_log2 * k0.x, m1 = 16.f * a.scale_log2 * k1.x;
-      const float c0 = fmaf(a.scale_log2, k0.y, -m0), c1 = fmaf(a.scale_log2, k1.y, -m1);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        s[nt][kb][0] = fmaf(s[nt][kb][0], m0, c0 * sumq[nt][0]);
-        s[nt][kb][1] = fmaf(s[nt][kb][1], m0, c0 * sumq[nt][1]);
-        s[nt][kb][2] = fmaf(s[nt][kb][2], m1, c1 * sumq[nt][0]);
-        s[nt][kb][3] = fmaf(s[nt][kb][3], m1, c1 * sumq[nt][1]);
+        s[nt][kb][0] = fmaf(s[nt][kb][0], k0.x, k0.y * sumq[nt][0]);
+        s[nt][kb][1] = fmaf(s[nt][kb][1], k0.x, k0.y * sumq[nt][1]);
+        s[nt][kb][2] = fmaf(s[nt][kb][2], k1.x, k1.y * sumq[nt][0]);
+        s[nt][kb][3] = fmaf(s[nt][kb][3], k1.x, k1.y * sumq[nt][1]);
       }
       if (masked) {
 #pragma unroll
@@ -377,20 +503,20 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
         m = fmaxf(m, mx[nt][x]);
-        base[nt][x] = m == -INFINITY ? 0.f : m;
-        al[x] = ex2(mx[nt][x] - base[nt][x]);
+        base[nt][x] = m == -INFINITY ? 0.f : m * c1[nt][x];
+        al[x] = mx[nt][x] == m ? 1.f : ex2(fmaf(mx[nt][x], c1[nt][x], -base[nt][x]));
         mx[nt][x] = m;
       }
-      if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
+      if (__any_sync(0xffffffffu, al[0] * shrink != 1.f || al[1] * shrink != 1.f)) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           l[nt][x] *= al[x];
           low[nt][x] *= al[x];
-          ones[nt][x] *= al[x];
+          const float f = al[x] * shrink;
 #pragma unroll
           for (int d = 0; d < D / 16; ++d) {
-            o[nt][d][x] *= al[x];
-            o[nt][d][2 + x] *= al[x];
+            o[nt][d][x] *= f;
+            o[nt][d][2 + x] *= f;
           }
         }
       }
@@ -399,26 +525,27 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
     // ---- weights, and the output's products
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      const float2 v0 = unpack2<T>(vaff[16 * kb + g]), v1 = unpack2<T>(vaff[16 * kb + 8 + g]);
+      const float2 v0 = unpack2<T>(va[kb][0]), v1 = unpack2<T>(va[kb][1]);
+      const float f0 = v0.x * vf, f1 = v1.x * vf;
       uint32_t bf[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float pe = ex2(s[nt][kb][e] - base[nt][e & 1]);
-          const float2 va = e < 2 ? v0 : v1;
+          const float pe = ex2(fmaf(s[nt][kb][e], c1[nt][e & 1], -base[nt][e & 1]));
           l[nt][e & 1] += pe;
-          w[e] = pe * (M::kF * va.x);
-          float lo = pe * va.y;
-          // a key the row does not see may hold anything, NaN included
-          if (masked && s[nt][kb][e] == -INFINITY) w[e] = lo = 0.f;
-          low[nt][e & 1] += lo;
+          w[e] = pe * (e < 2 ? f0 : f1);
+          if (!masked) {
+            low[nt][e & 1] = fmaf(pe, e < 2 ? v0.y : v1.y, low[nt][e & 1]);
+          } else if (s[nt][kb][e] == -INFINITY) {
+            w[e] = 0.f;  // a key this row does not see may be NaN to others
+          } else {
+            low[nt][e & 1] = fmaf(pe, e < 2 ? v0.y : v1.y, low[nt][e & 1]);
+          }
         }
-        bf[nt][0] = movmatrix_trans(pack2<T>(w[0], w[1]));
-        bf[nt][1] = movmatrix_trans(pack2<T>(w[2], w[3]));
-        const uint32_t one[4] = {M::kOne, M::kOne, M::kOne, M::kOne};
-        M::mma(ones[nt], one, bf[nt][0], bf[nt][1]);
+        bf[nt][0] = movmatrix_trans(pack2<__half>(w[0], w[1]));
+        bf[nt][1] = movmatrix_trans(pack2<__half>(w[2], w[3]));
       }
       // keys 2q, 2q + 1 and 2q + 8, 2q + 9 of the block; D/8 dims from D/8 * g
       const uint8_t* vr = st + C::kCodes + (16 * kb + 2 * q) * (D / 2) + g * (D / 16);
@@ -438,25 +565,22 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
         // elements 0..3 (then 4..7) of the word, keys 2q | 2q + 1 and 2q + 8 | 2q + 9
         const uint32_t e0 = __byte_perm(x[0][w], x[1][w], 0x5410), e1 = __byte_perm(x[2][w], x[3][w], 0x5410);
         const uint32_t f0 = __byte_perm(x[0][w], x[1][w], 0x7632), f1 = __byte_perm(x[2][w], x[3][w], 0x7632);
-        const uint32_t a0[4] = {kv4_pair<T, 0>(e0), kv4_pair<T, 1>(e0), kv4_pair<T, 0>(e1), kv4_pair<T, 1>(e1)};
-        const uint32_t a1[4] = {kv4_pair<T, 2>(e0), kv4_pair<T, 3>(e0), kv4_pair<T, 2>(e1), kv4_pair<T, 3>(e1)};
-        const uint32_t a2[4] = {kv4_pair<T, 0>(f0), kv4_pair<T, 1>(f0), kv4_pair<T, 0>(f1), kv4_pair<T, 1>(f1)};
-        const uint32_t a3[4] = {kv4_pair<T, 2>(f0), kv4_pair<T, 3>(f0), kv4_pair<T, 2>(f1), kv4_pair<T, 3>(f1)};
+        const uint32_t g0 = e0 >> 8, g1 = e1 >> 8, h0 = f0 >> 8, h1 = f1 >> 8;
+        const uint32_t a0[4] = {e0 & kCode0, e0 & kCode1, e1 & kCode0, e1 & kCode1};
+        const uint32_t a1[4] = {g0 & kCode0, g0 & kCode1, g1 & kCode0, g1 & kCode1};
+        const uint32_t a2[4] = {f0 & kCode0, f0 & kCode1, f1 & kCode0, f1 & kCode1};
+        const uint32_t a3[4] = {h0 & kCode0, h0 & kCode1, h1 & kCode0, h1 & kCode1};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          M::mma(o[nt][4 * w + 0], a0, bf[nt][0], bf[nt][1]);
-          M::mma(o[nt][4 * w + 1], a1, bf[nt][0], bf[nt][1]);
-          M::mma(o[nt][4 * w + 2], a2, bf[nt][0], bf[nt][1]);
-          M::mma(o[nt][4 * w + 3], a3, bf[nt][0], bf[nt][1]);
+          mma_f16(o[nt][4 * w + 0], a0, bf[nt][0], bf[nt][1]);
+          mma_f16(o[nt][4 * w + 1], a1, bf[nt][0], bf[nt][1]);
+          mma_f16(o[nt][4 * w + 2], a2, bf[nt][0], bf[nt][1]);
+          mma_f16(o[nt][4 * w + 3], a3, bf[nt][0], bf[nt][1]);
         }
       }
     }
     __syncwarp();  // every lane has read the stage
-    if (fetched < count) {
-      fetch(stage);
-      ++fetched;
-      advance(pr, fetched < count);
-    }
+    if (fetched < count) fetch_next(stage);
     if (++stage == STAGES) stage = 0, parity ^= 1;
 
     const bool run_ends = c.t + 1 == c.s.tiles;
@@ -464,7 +588,8 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
       // ---- a run (or a piece of one) is done
       const bool whole = t0 == 0 && run_ends;
       const int slot = t0 > 0 ? 0 : 1;
-      float* dst = reinterpret_cast<float*>(slot == 0 ? first_all + warp * C::kPiece : ring);
+      float* dst = slot == 0 ? first_all + warp * C::kPiece : reinterpret_cast<float*>(ring);
+      const float back = pow2f(vexp);  // 2^-24 of the codes and 2^(14 - vexp) of the weights, undone in two steps
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -476,18 +601,17 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
             lw += __shfl_xor_sync(0xffffffffu, lw, sh);
           }
           const int row = nt * 8 + 2 * q + x, rr = r0 + row;
-          constexpr float f = 16.f / M::kF;
           const float inv = whole ? (ls == 0.f ? 0.f : 1.f / ls) : 1.f;
           float y[D / 8];
 #pragma unroll
           for (int d = 0; d < D / 16; ++d) {
-            y[2 * d] = fmaf(f, o[nt][d][x] - ones[nt][x], lw) * inv;
-            y[2 * d + 1] = fmaf(f, o[nt][d][2 + x] - ones[nt][x], lw) * inv;
+            y[2 * d] = fmaf(o[nt][d][x] * 0x1p10f, back, lw) * inv;
+            y[2 * d + 1] = fmaf(o[nt][d][2 + x] * 0x1p6f, back, lw) * inv;
           }
           if (whole) {
             if (rr < rows) {
               T* out = static_cast<T*>(a.out) +
-                       ((c.s.q0 + static_cast<int64_t>(rr / a.group)) * a.hq + c.h * a.group + rr % a.group) * D + g * (D / 8);
+                       ((c.s.q0 + static_cast<int64_t>(a.row_token(rr))) * a.hq + c.h * a.group + (rr - a.row_token(rr) * a.group)) * D + g * (D / 8);
 #pragma unroll
               for (int d = 0; d < D / 8; d += 8)
                 *reinterpret_cast<uint4*>(out + d) = make_uint4(pack2<T>(y[d], y[d + 1]), pack2<T>(y[d + 2], y[d + 3]),
@@ -498,7 +622,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
             for (int d = 0; d < D / 8; d += 4)
               *reinterpret_cast<float4*>(dst + row * D + g * (D / 8) + d) = make_float4(y[d], y[d + 1], y[d + 2], y[d + 3]);
             if (g == 0) {
-              dst[RB * D + row] = mx[nt][x];
+              dst[RB * D + row] = mx[nt][x] == -INFINITY ? -INFINITY : mx[nt][x] * c1[nt][x];
               dst[RB * D + RB + row] = ls;
             }
           }
@@ -513,6 +637,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
     }
     advance(c, i + 1 < count);
   }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining kernel may be set up
   if (failed) {  // a copy never came: let the others land (or give up on them too) before the memory goes
     for (int k = 0; k < STAGES; ++k) {
       if (++stage == STAGES) stage = 0, parity ^= 1;
@@ -538,59 +663,36 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
     d[0] = d[2] = 0;
   }
   __syncthreads();
-  for (int item = warp; item < runs * RB; item += WARPS) {
-    const int row = item % RB;
+  // A warp takes four rows of a run: a lane D/32 consecutive dims of each, pieces in order.
+  for (int item = warp; item < runs * (RB / 4); item += WARPS) {
+    const int row0 = item % (RB / 4) * 4;
     unsigned rest = open;
-    for (int k = item / RB; k; --k) rest &= rest - 1;
+    for (int k = item / (RB / 4); k; --k) rest &= rest - 1;
     const int head = __ffs(rest) - 1;
     const unsigned later = rest & (rest - 1);
     const unsigned group = all & ~((1u << head) - 1) & (later ? (later & -later) - 1 : ~0u);
-    const int tail = 31 - __clz(group);
-    auto data = [&](int i) {
-      return reinterpret_cast<const float*>(i & 1 ? kv4_smem + (i >> 1) * C::kRing : first_all + (i >> 1) * C::kPiece);
-    };
-    float m = -INFINITY;
-    for (unsigned x = group; x; x &= x - 1) m = fmaxf(m, data(__ffs(x) - 1)[RB * D + row]);
-    const float mb = m == -INFINITY ? 0.f : m;
-    float ls = 0.f, y[W4];
-#pragma unroll
-    for (int d = 0; d < W4; ++d) y[d] = 0.f;
+    Kv4Joined<D> y;
+    y.clear();
     for (unsigned x = group; x; x &= x - 1) {
-      const float* src = data(__ffs(x) - 1);
-      const float f = ex2(src[RB * D + row] - mb);
-      ls = fmaf(src[RB * D + RB + row], f, ls);
-#pragma unroll
-      for (int d = 0; d < W4; ++d) y[d] = fmaf(src[row * D + lane * W4 + d], f, y[d]);
+      const int i = __ffs(x) - 1;
+      y.add(i & 1 ? reinterpret_cast<const float*>(kv4_smem + (i >> 1) * C::kRing) : first_all + (i >> 1) * C::kPiece,
+            RB, row0, lane);
     }
     const int* hd = piece[head];
-    const bool starts = hd[1], ends = piece[tail][2];
+    const bool starts = hd[1], ends = piece[31 - __clz(group)][2];
     if (starts && ends) {
-      const Kv4Seq sq = kv4_seq<TILE, RB>(a, p.max_rows, hd[3]);
-      const int rr = hd[5] * RB + row;
-      if (rr < sq.n * a.group) {
-        T* out = static_cast<T*>(a.out) +
-                 ((sq.q0 + static_cast<int64_t>(rr / a.group)) * a.hq + hd[4] * a.group + rr % a.group) * D + lane * W4;
-        const float inv = ls == 0.f ? 0.f : 1.f / ls;
-#pragma unroll
-        for (int d = 0; d < W4; d += 2) *reinterpret_cast<uint32_t*>(out + d) = pack2<T>(y[d] * inv, y[d + 1] * inv);
-      }
+      y.template write<T>(a, kv4_seq<TILE, RB>(a, p.max_rows, hd[3]), hd[4], hd[5] * RB + row0, lane);
     } else {
       const int slot = starts ? 1 : 0;
-      float* dst = p.ws + (blockIdx.x * 2 + slot) * static_cast<int64_t>(RB * (D + 2));
-#pragma unroll
-      for (int d = 0; d < W4; ++d) dst[row * D + lane * W4 + d] = y[d];
-      if (lane == 0) {
-        dst[RB * D + row] = m;
-        dst[RB * D + RB + row] = ls;
-        if (row == 0) {
-          int* ds = p.desc + blockIdx.x * 8;
-          if (slot == 0) {
-            ds[1] = ends;
-            ds[0] = 1;
-          } else {
-            ds[3] = hd[3], ds[4] = hd[4], ds[5] = hd[5];
-            ds[2] = 1;
-          }
+      y.store(p.cta + (blockIdx.x * 2 + slot) * static_cast<int64_t>(C::kPiece), RB, row0, lane);
+      if (lane == 0 && row0 == 0) {
+        int* ds = p.desc + blockIdx.x * 8;
+        if (slot == 0) {
+          ds[1] = ends;
+          ds[0] = 1;
+        } else {
+          ds[3] = hd[3], ds[4] = hd[4], ds[5] = hd[5];
+          ds[2] = 1;
         }
       }
     }
@@ -598,50 +700,22 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
 }
 
 // Joins the pieces of the runs cut by CTA borders: CTA i takes the run that starts in (and runs out of) CTA
-// i of the first kernel. A warp per row, pieces in order.
+// i of the first kernel. A warp takes four rows.
 template <typename T, int D, int RB, int TILE>
-__global__ void __launch_bounds__(256) kv4_decode_join(const Kv4DecodeParams p, int parts) {
-  constexpr int W4 = D / 32;
-  const Kv4AttnParams& a = p.a;
+__global__ void __launch_bounds__(32 * RB / 4) kv4_decode_join(const Kv4DecodeParams p, int parts) {
+  constexpr int64_t kPiece = RB * (D + 2);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // until the first kernel is done and its stores are visible
   const int* d0 = p.desc + blockIdx.x * 8;
   if (!d0[2]) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int last = blockIdx.x;
-  for (int i = blockIdx.x + 1; i < parts; ++i) {
-    if (!p.desc[i * 8]) break;
-    last = i;
+  const int row0 = (threadIdx.x >> 5) * 4, lane = threadIdx.x & 31;
+  Kv4Joined<D> y;
+  y.clear();
+  y.add(p.cta + (blockIdx.x * 2 + 1) * kPiece, RB, row0, lane);
+  for (int i = blockIdx.x + 1; i < parts && p.desc[i * 8]; ++i) {
+    y.add(p.cta + i * 2 * kPiece, RB, row0, lane);
     if (p.desc[i * 8 + 1]) break;
   }
-  auto data = [&](int i) {
-    return p.ws + (i * 2 + (i == static_cast<int>(blockIdx.x) ? 1 : 0)) * static_cast<int64_t>(RB * (D + 2));
-  };
-  const int b = d0[3], h = d0[4], blk = d0[5];
-  const Kv4Seq sq = kv4_seq<TILE, RB>(a, p.max_rows, b);
-  for (int row = warp; row < RB; row += 8) {
-    const int rr = blk * RB + row;
-    if (rr >= sq.n * a.group) break;
-    float m = -INFINITY;
-    for (int i = blockIdx.x + lane; i <= last; i += 32) m = fmaxf(m, data(i)[RB * D + row]);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float mb = m == -INFINITY ? 0.f : m;
-    float ls = 0.f, y[W4];
-#pragma unroll
-    for (int d = 0; d < W4; ++d) y[d] = 0.f;
-#pragma unroll 4
-    for (int i = blockIdx.x; i <= last; ++i) {
-      const float* src = data(i);
-      const float f = ex2(src[RB * D + row] - mb);
-      ls = fmaf(src[RB * D + RB + row], f, ls);
-#pragma unroll
-      for (int d = 0; d < W4; ++d) y[d] = fmaf(src[row * D + lane * W4 + d], f, y[d]);
-    }
-    const float inv = ls == 0.f ? 0.f : 1.f / ls;
-    T* out = static_cast<T*>(a.out) +
-             ((sq.q0 + static_cast<int64_t>(rr / a.group)) * a.hq + h * a.group + rr % a.group) * D + lane * W4;
-#pragma unroll
-    for (int d = 0; d < W4; d += 2) *reinterpret_cast<uint32_t*>(out + d) = pack2<T>(y[d] * inv, y[d + 1] * inv);
-  }
+  y.template write<T>(p.a, kv4_seq<TILE, RB>(p.a, p.max_rows, d0[3]), d0[4], d0[5] * RB + row0, lane);
 }
 
 }  // namespace dscq
