@@ -500,7 +500,9 @@ bool rows_ok(const void* p, int64_t st, int64_t sh) { return p && aligned(p, 16)
 template <typename T, int D>
 cudaError_t launch_kv4_append(const dscq::Kv4AppendParams& p, bool f32, cudaStream_t st) {
   const int rows = p.hq + 2 * p.b.hk, per = dscq::Kv4Rows<D>::kPerCta;
-  const dim3 grid(static_cast<unsigned>(p.T), static_cast<unsigned>((rows + per - 1) / per));
+  // rows of a token spread over CTAs until the tokens fill the GPU: then a thread keeps its angles for all its rows
+  const int slices = p.T >= 8 * num_sms() ? 1 : (rows + per - 1) / per;
+  const dim3 grid(static_cast<unsigned>(p.T), static_cast<unsigned>(slices));
   if (f32)
     dscq::kv4_append_kernel<T, D, true><<<grid, 256, 0, st>>>(p);
   else
@@ -1246,17 +1248,25 @@ int dscq_token_logprobs(const void* logits, int x_dtype, int64_t rows, int64_t V
   DSCQ_REQUIRE(aligned(logits, x_dtype == DSCQ_F32 ? 4 : 2), "logits must be aligned to their type");
   int st = check_device(nullptr);
   if (st) return st;
-  dscq::LogprobParams p{logits, targets, logprobs, entropy, top_logprobs, top_ids,
-                        ld,     static_cast<int>(rows), static_cast<int>(V), k};
-  cudaStream_t cst = static_cast<cudaStream_t>(stream);
-  const unsigned grid = static_cast<unsigned>(rows);
-  if (x_dtype == DSCQ_BF16)
-    dscq::logprob_rows<__nv_bfloat16><<<grid, 256, 0, cst>>>(p);
-  else if (x_dtype == DSCQ_F16)
-    dscq::logprob_rows<__half><<<grid, 256, 0, cst>>>(p);
-  else
-    dscq::logprob_rows<float><<<grid, 256, 0, cst>>>(p);
-  cudaError_t e = cudaGetLastError();
+  // Few rows are cut into slices, a cluster a row, until there are two CTAs an SM; a slice keeps 2048 logits.
+  int parts = 1;
+  while (parts < 8 && rows * parts < num_sms() * 2 && V / (2 * parts) >= 2048) parts *= 2;
+  const dscq::LogprobParams p{logits, targets, logprobs, entropy, top_logprobs, top_ids, ld, static_cast<int>(rows),
+                              static_cast<int>(V), k, parts};
+  DSCQ_REQUIRE(rows * parts < (int64_t(1) << 31), "too many rows");
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = static_cast<unsigned>(parts);
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * parts));
+  cfg.blockDim = dim3(dscq::kLpThreads);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cfg.attrs = &cluster;
+  cfg.numAttrs = parts > 1 ? 1 : 0;
+  cudaError_t e = x_dtype == DSCQ_BF16  ? cudaLaunchKernelEx(&cfg, dscq::logprob_rows<__nv_bfloat16>, p)
+                  : x_dtype == DSCQ_F16 ? cudaLaunchKernelEx(&cfg, dscq::logprob_rows<__half>, p)
+                                        : cudaLaunchKernelEx(&cfg, dscq::logprob_rows<float>, p);
   if (e != cudaSuccess) return cuda_fail(e, "launch token_logprobs");
   return DSCQ_OK;
 }

@@ -13,6 +13,8 @@
 // min and low are taken on the unrounded (rotated) row: rounding it to 16 bits first would cost up to half a
 // 16-bit step on every element for nothing, since only codes are kept.
 #pragma once
+#include <type_traits>
+
 #include "ptx.cuh"
 
 namespace dscq {
@@ -126,146 +128,288 @@ __device__ __forceinline__ void kv4_unpack8(const uint4& w, float (&f)[8]) {
   }
 }
 
-template <bool F32, typename T>
-__device__ __forceinline__ void kv4_table8(const void* tab, int64_t at, float (&f)[8]) {
-  if constexpr (F32) {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(tab) + at);
-    const float4 a = p[0], b = p[1];
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-  } else {
-    kv4_unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(tab) + at), f);
+// Eight entries of an angle table, kept as they are stored.
+template <typename T, bool F32>
+struct Kv4Angles {
+  uint4 w[F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* table, int64_t at) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(table) + at * (F32 ? 4 : 2));
+    w[0] = p[0];
+    if constexpr (F32) w[1] = p[1];
   }
-}
-
-// Code of y in [low, ...] with the given step (> 0, finite). The quotient in 32 bits decides except within
-// 2^-10 of the border of two codes (the quotient's error is below 2^-19), where the sign of the exact
-// difference in 64 bits does; a tie goes to the even code.
-template <typename Y>
-__device__ __forceinline__ uint32_t kv4_code(Y y, float low, float step, float inv) {
-  const float t = static_cast<float>(y - static_cast<Y>(low)) * inv;
-  float c = rintf(t);
-  if (fabsf(fabsf(t - c) - 0.5f) < 0x1p-10f) {
-    const double below = floor(static_cast<double>(t));
-    const double d = (static_cast<double>(y) - low) - (below + 0.5) * static_cast<double>(step);
-    const bool odd = (static_cast<int>(below) & 1) != 0;
-    c = static_cast<float>(below) + ((d > 0 || (d == 0 && odd)) ? 1.f : 0.f);
+  __device__ __forceinline__ float get(int i) const {  // i is a constant once unrolled
+    const uint4 v = w[F32 ? i / 4 : 0];
+    const int j = F32 ? i % 4 : i / 2;
+    const uint32_t x = j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
+    if constexpr (F32) return __uint_as_float(x);
+    const float2 f = unpack2<T>(x);
+    return i % 2 ? f.y : f.x;
   }
-  return static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f));
-}
+};
 
-// Quantises the row whose elements this lane group holds (ya: 8 of the first half, yb: 8 of the second) and
-// stores it. Every lane of the warp takes part in the shuffles.
-template <typename T, int D, typename Y>
-__device__ __forceinline__ void kv4_store_row(const Y (&ya)[8], const Y (&yb)[8], uint8_t* codes, uint32_t* affine,
-                                              int64_t row, int j0, bool store) {
-  Y mn = ya[0], mx = ya[0];
+// The rows' definition in 64 bits, for the whole warp: low, step and the codes of the 16 elements of this lane, x[0..7]
+// and x[D/2 ..], rotated with the angles at `at` unless cos is null.
+struct Kv4Row {
+  float low, step;
+  uint32_t wa, wb;
+};
+template <typename T, int D, bool F32>
+__device__ __forceinline__ Kv4Row kv4_quantise_exact(const T* x, const void* cos, const void* sin, int64_t at) {
+  constexpr int H = D / 2;
+  double y[16];
+  {
+    float a[8], b[8];
+    kv4_unpack8<T>(*reinterpret_cast<const uint4*>(x), a);
+    kv4_unpack8<T>(*reinterpret_cast<const uint4*>(x + H), b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = a[i], y[i + 8] = b[i];
+    if (cos) {
+      Kv4Angles<T, F32> c, s;
+      c.load(cos, at);
+      s.load(sin, at);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        y[i] = static_cast<double>(a[i]) * c.get(i) - static_cast<double>(b[i]) * s.get(i);
+      c.load(cos, at + H);
+      s.load(sin, at + H);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        y[i + 8] = static_cast<double>(b[i]) * c.get(i) + static_cast<double>(a[i]) * s.get(i);
+    }
+  }
+  double mn = y[0], mx = y[0];
   bool nan = false;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    mn = min(mn, min(ya[i], yb[i]));
-    mx = max(mx, max(ya[i], yb[i]));
-    nan |= ya[i] != ya[i] || yb[i] != yb[i];  // min and max drop a NaN
+  for (int i = 0; i < 16; ++i) {
+    mn = y[i] < mn ? y[i] : mn;
+    mx = y[i] > mx ? y[i] : mx;
+    nan |= y[i] != y[i];
   }
 #pragma unroll
   for (int o = Kv4Rows<D>::kLanes / 2; o; o >>= 1) {
-    mn = min(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const double n = __shfl_xor_sync(0xffffffffu, mn, o), x2 = __shfl_xor_sync(0xffffffffu, mx, o);
+    mn = n < mn ? n : mn;
+    mx = x2 > mx ? x2 : mx;
     nan |= __shfl_xor_sync(0xffffffffu, static_cast<int>(nan), o) != 0;
   }
-  const float low = to_float<T>(from_float<T>(static_cast<float>(mn)));
-  const float step = to_float<T>(from_float<T>(static_cast<float>((static_cast<double>(mx) - low) / 15.0)));
-  const bool bad = nan || !isfinite(low) || !isfinite(step);
-  uint32_t wa = 0, wb = 0;
-  if (!bad && step != 0.f) {
-    const float inv = 1.f / step;
-    if (isfinite(inv)) {
+  Kv4Row r;
+  r.low = to_float<T>(from_float<T>(static_cast<float>(mn)));
+  r.step = to_float<T>(from_float<T>(static_cast<float>((mx - r.low) / 15.0)));
+  r.wa = r.wb = 0;
+  if (nan || !isfinite(r.low) || !isfinite(r.step)) {
+    r.low = r.step = __int_as_float(0x7fc00000);
+  } else if (r.step != 0.f) {
+    const double low = r.low, step = r.step, inv = 1.0 / step;
+    bool close = false;
+    auto pack = [&](auto quotient) {
+      r.wa = r.wb = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        wa |= kv4_code<Y>(ya[i], low, step, inv) << (4 * i);
-        wb |= kv4_code<Y>(yb[i], low, step, inv) << (4 * i);
+        r.wa |= static_cast<uint32_t>(quotient(y[i] - low)) << (4 * i);
+        r.wb |= static_cast<uint32_t>(quotient(y[i + 8] - low)) << (4 * i);
       }
-    } else {  // a step so small that its reciprocal overflows: divide in 64 bits
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const double a = rint((static_cast<double>(ya[i]) - low) / step), b = rint((static_cast<double>(yb[i]) - low) / step);
-        wa |= static_cast<uint32_t>(fmin(fmax(a, 0.0), 15.0)) << (4 * i);
-        wb |= static_cast<uint32_t>(fmin(fmax(b, 0.0), 15.0)) << (4 * i);
-      }
-    }
+    };
+    pack([&](double d) {
+      const double t = d * inv, c = rint(t);
+      close |= fabs(fabs(t - c) - 0.5) < 0x1p-40;
+      return c < 0.0 ? 0.0 : c > 15.0 ? 15.0 : c;
+    });
+    if (close)  // next to a border the quotient itself decides
+      pack([&](double d) { return fmin(fmax(rint(d / step), 0.0), 15.0); });
   }
-  if (!store) return;
-  uint8_t* c = codes + row * (D / 2) + j0 / 2;
-  *reinterpret_cast<uint32_t*>(c) = wa;
-  *reinterpret_cast<uint32_t*>(c + D / 4) = wb;
-  const float nanv = __int_as_float(0x7fc00000);
-  if (j0 == 0) affine[row] = pack2<T>(bad ? nanv : step, bad ? nanv : low);
+  return r;
 }
 
-// grid (T, ceil((hq + 2 hk) / rows per CTA)), 256 threads. A group of D/16 lanes takes one row: q rows are
-// rotated in 32 bits and rounded once; k rows are rotated in 64 bits (the products and their sum are exact
-// there, so codes do not depend on how a compiler contracts them) and quantised; v rows are quantised.
+// Largest (smallest) of three, NaN if one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// The same in 32 bits for the 16 elements of this lane. `exact`: they are 16-bit numbers; otherwise they are off by
+// at most `rel` times the larger of their own size and `big`. False where that, or the rounding of the arithmetic,
+// could decide low, step or a code otherwise than 64 bits do, and where a row is not plain numbers.
+//
+// Borders of two codes. Inexact rows: no quotient may lie within a window of one. Exact rows are full of ties, which
+// rint sends to the even code as it should once the quotient is rounded correctly (one Newton step). A quotient that
+// is not a tie stays clear of the border: elements of at least 2^-C of the row's largest are multiples of a power of
+// two for which the distance is over 2^-19 (C = 14 for 8 mantissa bits; 11 bits leave 10), and smaller elements sit
+// within 2^(4 - C) of the quotient of 0, which must not be near a border itself.
+// Codes come out of the rounding addition: the low bits of 1.5 2^23 + t are rint(t).
+template <typename T, int D>
+__device__ __forceinline__ bool kv4_quantise_fast(const float (&ya)[8], const float (&yb)[8], bool exact, float big,
+                                                  float rel, Kv4Row& out) {
+  constexpr float kMagic = 12582912.f;
+  float mn = ya[0], mx = ya[0];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    mn = min3(mn, ya[i], yb[i]);
+    mx = max3(mx, ya[i], yb[i]);
+  }
+#pragma unroll
+  for (int o = Kv4Rows<D>::kLanes / 2; o; o >>= 1) {
+    const float n = __shfl_xor_sync(0xffffffffu, mn, o), x = __shfl_xor_sync(0xffffffffu, mx, o);
+    mn = min3(mn, n, n);
+    mx = max3(mx, x, x);
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+  }
+  const float low = to_float<T>(from_float<T>(mn)), range = mx - low;
+  const float step = to_float<T>(from_float<T>(__fdiv_rn(range, 15.f))), inv = 1.f / step;
+  out.low = low;
+  out.step = step;
+  // false for NaN and infinities, a step of 0 or one whose reciprocal overflows, and codes outside 0 .. 15
+  bool ok = range * inv < 15.4f && (mn - low) * inv > -0.4f && inv < INFINITY;
+  uint32_t wa = 0, wb = 0;
+  if (exact) {
+    const float back = range - mx;  // the range must not have been rounded
+    ok = ok && (mx - (range - back)) + (-low - back) == 0.f;
+    auto quotient = [&](float y) {
+      const float d = y - low, t = d * inv;
+      return fmaf(fmaf(-t, step, d), inv, t);
+    };
+    constexpr float kNear = std::is_same<T, __half>::value ? 0x1p-6f : 0x1p-10f;
+    const float zero = quotient(0.f);
+    ok = ok && (mn > 0.f || mx < 0.f || 0.5f - fabsf(zero - rintf(zero)) > kNear);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      wa += __float_as_uint(quotient(ya[i]) + kMagic) << (4 * i);
+      wb += __float_as_uint(quotient(yb[i]) + kMagic) << (4 * i);
+    }
+  } else {
+    const float err = fmaxf(big, fmaxf(fabsf(mn), fabsf(mx))) * rel, slack = err + fabsf(range) * 0x1p-22f;
+    ok = ok && low == to_float<T>(from_float<T>(mn - err)) && low == to_float<T>(from_float<T>(mn + err)) &&
+         step == to_float<T>(from_float<T>((range - slack) * (1.f / 15.f))) &&
+         step == to_float<T>(from_float<T>((range + slack) * (1.f / 15.f)));
+    const float shift = -low * inv;
+    // y inv + shift is off by the element's error, that of inv and the roundings of shift and of the result
+    const float window = 0x1p-19f + (2.f * err + 0x1p-22f * fmaxf(fabsf(mn), fabsf(mx))) * fabsf(inv);
+    float far = 0.f;
+    auto code = [&](float y) {
+      const float t = fmaf(y, inv, shift), r = t + kMagic;
+      far = fmaxf(far, fabsf(t - (r - kMagic)));
+      return __float_as_uint(r);
+    };
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      wa += code(ya[i]) << (4 * i);
+      wb += code(yb[i]) << (4 * i);
+    }
+    ok = ok && far < 0.5f - window;
+  }
+  constexpr uint32_t kBias = 0x4B400000u + (0x4B400000u << 4) + (0x4B400000u << 8);  // the rest shifts out
+  out.wa = wa - kBias;
+  out.wb = wb - kBias;
+  return ok;
+}
+
+// One CTA per token and 256-thread slice of its hq + 2 hk rows (gridDim.y slices; fewer, with more rows a thread,
+// once the tokens alone fill the GPU). A group of D/16 lanes takes one row: q rows are rotated in 32 bits and
+// rounded once; k rows are rotated and quantised in 32 bits with a bound on the error, and again in 64 bits where
+// that could change a bit, so codes are those of the definition; v rows likewise, from exact values.
 // Bound by HBM at many rows: q in and out, k and v in, an eighth of that out as codes.
 template <typename T, int D, bool F32>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p) {
+__global__ void __launch_bounds__(256, 3) kv4_append_kernel(const Kv4AppendParams p) {
   using R = Kv4Rows<D>;
   constexpr int H = D / 2;
-  const int t = blockIdx.x;
-  const int r = blockIdx.y * R::kPerCta + threadIdx.x / R::kLanes;
+  const int t = blockIdx.x, hk = p.b.hk, rows = p.hq + 2 * hk;
   const int j0 = (threadIdx.x % R::kLanes) * 8;
-  const int hk = p.b.hk;
-  const int kind = r < p.hq ? 0 : r < p.hq + hk ? 1 : r < p.hq + 2 * hk ? 2 : 3;
-  const int h = kind == 0 ? r : kind == 1 ? r - p.hq : r - p.hq - hk;
-  uint4 xa = make_uint4(0, 0, 0, 0), xb = xa;
-  if (kind < 3) {
-    const T* src = static_cast<const T*>(kind == 0 ? p.q : kind == 1 ? p.k : p.v) +
-                   t * (kind == 0 ? p.q_t : kind == 1 ? p.k_t : p.v_t) +
-                   h * (kind == 0 ? p.q_h : kind == 1 ? p.k_h : p.v_h) + j0;
-    xa = *reinterpret_cast<const uint4*>(src);
-    xb = *reinterpret_cast<const uint4*>(src + H);
-  }
+  // every lane of a warp runs the same rounds: the shuffles need them all
+  const int first = blockIdx.y * R::kPerCta + threadIdx.x / R::kLanes;
+  int r = first;
+  const int rounds = (rows - static_cast<int>(blockIdx.y) * R::kPerCta + gridDim.y * R::kPerCta - 1) /
+                     static_cast<int>(gridDim.y * R::kPerCta);
+  uint4 xa, xb;  // the round's row, and the next one's on their way
+  uint4 na, nb;
+  auto row_of = [&](int row) {
+    return j0 + (row < p.hq        ? static_cast<const T*>(p.q) + t * p.q_t + row * p.q_h
+                 : row < p.hq + hk ? static_cast<const T*>(p.k) + t * p.k_t + (row - p.hq) * p.k_h
+                                   : static_cast<const T*>(p.v) + t * p.v_t + (row - p.hq - hk) * p.v_h);
+  };
+  auto load = [&](int row) {
+    na = nb = make_uint4(0, 0, 0, 0);
+    if (row >= rows) return;
+    const T* src = row_of(row);
+    na = *reinterpret_cast<const uint4*>(src);
+    nb = *reinterpret_cast<const uint4*>(src + H);
+  };
+  load(r);
   Kv4Where w = kv4_where(p.b, t);
   if (w.seq >= 0 && !w.bad && w.pos >= p.table_rows) w.bad = true;
   if (w.bad && threadIdx.x == 0) raise_status(kStatusBadIndex);
   const bool real = w.seq >= 0 && !w.bad;
-  float a[8], b[8], ca[8], cb[8], sa[8], sb[8];
-  kv4_unpack8<T>(xa, a);
-  kv4_unpack8<T>(xb, b);
-  const int64_t at = static_cast<int64_t>(real ? w.pos : 0) * D + j0;
-  if (kind < 2 && real) {
-    kv4_table8<F32, T>(p.cos, at, ca);
-    kv4_table8<F32, T>(p.cos, at + H, cb);
-    kv4_table8<F32, T>(p.sin, at, sa);
-    kv4_table8<F32, T>(p.sin, at + H, sb);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ca[i] = cb[i] = sa[i] = sb[i] = 0.f;
+  Kv4Angles<T, F32> cos_a, cos_b, sin_a, sin_b;
+  if (real) {
+    const int64_t at = static_cast<int64_t>(w.pos) * D + j0;
+    cos_a.load(p.cos, at);
+    cos_b.load(p.cos, at + H);
+    sin_a.load(p.sin, at);
+    sin_b.load(p.sin, at + H);
   }
-  if (kind == 0) {
-    uint32_t oa[4], ob[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int e = 2 * i;
-      oa[i] = real ? pack2<T>(a[e] * ca[e] - b[e] * sa[e], a[e + 1] * ca[e + 1] - b[e + 1] * sa[e + 1]) : 0u;
-      ob[i] = real ? pack2<T>(b[e] * cb[e] + a[e] * sb[e], b[e + 1] * cb[e + 1] + a[e + 1] * sb[e + 1]) : 0u;
+  const int64_t slot = w.pos & ((1 << p.b.ps_log2) - 1);
+  auto store = [&](int row, const Kv4Row& y) {
+    const bool is_k = row < p.hq + hk;
+    const int64_t at = ((w.page * hk + (row - p.hq - (is_k ? 0 : hk))) << p.b.ps_log2) + slot;
+    uint8_t* c = (is_k ? p.b.kc : p.b.vc) + at * (D / 2) + j0 / 2;
+    *reinterpret_cast<uint32_t*>(c) = y.wa;
+    *reinterpret_cast<uint32_t*>(c + D / 4) = y.wb;
+    if (j0 == 0) (is_k ? p.b.ka : p.b.va)[at] = pack2<T>(y.step, y.low);
+  };
+  bool again = false;
+  for (int round = 0; round < rounds; ++round, r += gridDim.y * R::kPerCta) {
+    xa = na, xb = nb;
+    if (round + 1 < rounds) load(r + gridDim.y * R::kPerCta);
+    const bool is_q = r < p.hq, is_k = !is_q && r < p.hq + hk, is_v = r >= p.hq + hk && r < rows;
+    if (!real) {  // the whole CTA: nothing to cache, zero queries
+      if (is_q) {
+        T* o = static_cast<T*>(p.q_out) + (static_cast<int64_t>(t) * p.hq + r) * D + j0;
+        *reinterpret_cast<uint4*>(o) = *reinterpret_cast<uint4*>(o + H) = make_uint4(0, 0, 0, 0);
+      }
+      continue;
     }
-    T* o = static_cast<T*>(p.q_out) + (static_cast<int64_t>(t) * p.hq + h) * D + j0;
-    *reinterpret_cast<uint4*>(o) = make_uint4(oa[0], oa[1], oa[2], oa[3]);
-    *reinterpret_cast<uint4*>(o + H) = make_uint4(ob[0], ob[1], ob[2], ob[3]);
-  }
-  const bool store = real && (kind == 1 || kind == 2);
-  const int64_t row = ((w.page * hk + h) << p.b.ps_log2) + (w.pos & ((1 << p.b.ps_log2) - 1));
-  if (__any_sync(0xffffffffu, store && kind == 1)) {
-    double ya[8], yb[8];
+    float ya[8], yb[8], big = 0.f;
+    kv4_unpack8<T>(xa, ya);
+    kv4_unpack8<T>(xb, yb);
+    if (!is_v) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const double x1 = a[i], x2 = b[i];
-      ya[i] = x1 * static_cast<double>(ca[i]) - x2 * static_cast<double>(sa[i]);
-      yb[i] = x2 * static_cast<double>(cb[i]) + x1 * static_cast<double>(sb[i]);
+      for (int i = 0; i < 8; ++i) {
+        const float x = ya[i], ua = yb[i] * sin_a.get(i), ub = x * sin_b.get(i);
+        ya[i] = fmaf(x, cos_a.get(i), -ua);
+        yb[i] = fmaf(yb[i], cos_b.get(i), ub);
+        if constexpr (F32) big = fmaxf(big, fmaxf(fabsf(ua), fabsf(ub)));
+      }
     }
-    kv4_store_row<T, D, double>(ya, yb, p.b.kc, p.b.ka, row, j0, store && kind == 1);
+    if (is_q) {
+      T* o = static_cast<T*>(p.q_out) + (static_cast<int64_t>(t) * p.hq + r) * D + j0;
+      *reinterpret_cast<uint4*>(o) = make_uint4(pack2<T>(ya[0], ya[1]), pack2<T>(ya[2], ya[3]), pack2<T>(ya[4], ya[5]),
+                                                pack2<T>(ya[6], ya[7]));
+      *reinterpret_cast<uint4*>(o + H) = make_uint4(pack2<T>(yb[0], yb[1]), pack2<T>(yb[2], yb[3]),
+                                                    pack2<T>(yb[4], yb[5]), pack2<T>(yb[6], yb[7]));
+    }
+    if (!__any_sync(0xffffffffu, is_k || is_v)) continue;
+    Kv4Row y;
+    // the sum rounds by 2^-24 of itself; products of 16-bit numbers are exact, those with a 32-bit angle are not
+    const bool ok = kv4_quantise_fast<T, D>(ya, yb, is_v, big, F32 ? 0x1p-23f : 0x1p-24f, y);
+    again |= !ok && (is_k || is_v);
+    if (is_k || is_v) store(r, y);
   }
-  if (__any_sync(0xffffffffu, store && kind == 2))
-    kv4_store_row<T, D, float>(a, b, p.b.vc, p.b.va, row, j0, store && kind == 2);
+  // Seldom: 64 bits for the warp's rows. Behind the loop, where nothing else needs the registers.
+  if (real && __any_sync(0xffffffffu, again)) {
+    r = first;
+#pragma unroll 1
+    for (int round = 0; round < rounds; ++round, r += gridDim.y * R::kPerCta) {
+      const bool is_k = r >= p.hq && r < p.hq + hk, cached = r >= p.hq && r < rows;
+      if (!__any_sync(0xffffffffu, cached)) continue;
+      const Kv4Row y = kv4_quantise_exact<T, D, F32>(row_of(min(r, rows - 1)), is_k ? p.cos : nullptr, p.sin,
+                                                     static_cast<int64_t>(w.pos) * D + j0);
+      if (cached) store(r, y);
+    }
+  }
 }
 
 // The values the cache holds for the rows of the token axis, [T, hk, D] each; zero rows where a row belongs

@@ -22,19 +22,21 @@ class PagedKV4:
 
     def __post_init__(self) -> None:
         c, a = self.k_codes, self.k_affine
-        if c.dim() != 4 or c.shape[3] not in (32, 64):
+        shape = c.shape
+        if len(shape) != 4 or shape[3] not in (32, 64):
             raise RuntimeError("codes must be [pages, kv_heads, page_size, head_dim / 2] with head_dim 64 or 128")
-        ps = c.shape[2]
+        ps = shape[2]
         if ps < 16 or ps > 1024 or ps & (ps - 1):
             raise RuntimeError("page_size must be a power of two from 16 to 1024")
-        if a.dtype not in (torch.bfloat16, torch.float16) or self.v_affine.dtype != a.dtype:
-            raise RuntimeError("affine must be bf16 or f16, the same for keys and values")
-        for codes, affine in ((c, a), (self.v_codes, self.v_affine)):
-            if codes.dtype != torch.uint8 or codes.shape != c.shape or affine.shape != (*c.shape[:3], 2):
-                raise RuntimeError("codes must be uint8, affine [pages, kv_heads, page_size, 2]")
-            for t in (codes, affine):
-                if not t.is_cuda or t.device != c.device or not t.is_contiguous():
-                    raise RuntimeError("the cache's tensors must be contiguous CUDA tensors on one device")
+        if a.dtype not in (torch.bfloat16, torch.float16):
+            raise RuntimeError("affine must be bf16 or f16")
+        pairs = (*shape[:3], 2)
+        for t, want, dtype in ((c, shape, torch.uint8), (self.v_codes, shape, torch.uint8), (a, pairs, a.dtype),
+                               (self.v_affine, pairs, a.dtype)):
+            if t.shape != want or t.dtype != dtype:
+                raise RuntimeError("codes must be uint8 and alike, affine [pages, kv_heads, page_size, 2] of one type")
+            if not t.is_cuda or t.device != c.device or not t.is_contiguous():
+                raise RuntimeError("the cache's tensors must be contiguous CUDA tensors on one device")
 
     @classmethod
     def allocate(cls, pages: int, kv_heads: int, head_dim: int, page_size: int = 64,

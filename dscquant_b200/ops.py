@@ -34,6 +34,15 @@ def _stream(device: torch.device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def _launch(dev: torch.device, fn, *args) -> int:
+    """fn(*args, stream) on `dev`'s current stream. The raw handle and the test for the current device cost a
+    fraction of a microsecond, a device context and a Stream object about eight."""
+    if torch.cuda.current_device() == dev.index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    with torch.cuda.device(dev):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+
+
 def _check_cuda(t: torch.Tensor, name: str) -> None:
     if not (t.is_cuda and t.is_contiguous()):
         raise RuntimeError(f"Expected contiguous CUDA tensor for {name}")
@@ -409,31 +418,33 @@ def _no_grad_inputs(*tensors: torch.Tensor) -> None:
 def _kv4_batch(cache: PagedKV4, page_table: torch.Tensor, q_start: torch.Tensor, lengths: torch.Tensor):
     """The dscq_kv4_batch of a call, after the checks every cache operator makes."""
     dev = cache.device
-    for name, t in (("page_table", page_table), ("q_start", q_start), ("lengths", lengths)):
-        if t.dtype != torch.int32 or t.device != dev:
-            raise RuntimeError(f"{name} must be an int32 tensor on {dev}")
-    B = lengths.numel()
-    if lengths.dim() != 1 or q_start.dim() != 1 or q_start.numel() != B + 1:
+    if not (page_table.dtype == q_start.dtype == lengths.dtype == torch.int32 and
+            page_table.device == q_start.device == lengths.device == dev):
+        raise RuntimeError(f"page_table, q_start and lengths must be int32 tensors on {dev}")
+    if lengths.dim() != 1 or q_start.shape != (lengths.shape[0] + 1,):
         raise RuntimeError("need lengths [B] and q_start [B + 1]")
+    B = lengths.shape[0]
     if page_table.dim() != 2 or page_table.shape[0] != B:
         raise RuntimeError("page_table must be [B, pages]")
-    if (B > 1 and (lengths.stride(0) != 1 or page_table.stride(0) < page_table.shape[1])) or \
-            (B and q_start.stride(0) != 1) or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+    P, ld = page_table.shape[1], page_table.stride(0)
+    if (P > 1 and page_table.stride(1) != 1) or (B and q_start.stride(0) != 1) or \
+            (B > 1 and (ld < P or lengths.stride(0) != 1)):
         raise RuntimeError("page_table rows, q_start and lengths must be contiguous")
-    pages, hk, ps, half = cache.k_codes.shape
-    P = page_table.shape[1]
-    return _lib.Kv4Batch(cache.k_codes.data_ptr(), cache.k_affine.data_ptr(), cache.v_codes.data_ptr(),
+    codes = cache.k_codes
+    pages, hk, ps, half = codes.shape
+    return _lib.Kv4Batch(codes.data_ptr(), cache.k_affine.data_ptr(), cache.v_codes.data_ptr(),
                          cache.v_affine.data_ptr(), pages, hk, ps, half * 2, _DT[cache.dtype],
-                         page_table.data_ptr(), max(page_table.stride(0), P), P, q_start.data_ptr(),
-                         lengths.data_ptr(), B)
+                         page_table.data_ptr(), max(ld, P), P, q_start.data_ptr(), lengths.data_ptr(), B)
 
 
 def _kv4_rows(cache: PagedKV4, name: str, t: torch.Tensor, T: int, heads: int | None) -> None:
-    if t.dim() != 3 or t.shape[0] != T or t.shape[2] != cache.head_dim or (heads is not None and t.shape[1] != heads):
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != T or shape[2] != cache.head_dim or (heads is not None and shape[1] != heads):
         raise RuntimeError(f"{name} must be [{T}, {heads or 'heads'}, {cache.head_dim}]")
     if t.dtype != cache.dtype or t.device != cache.device:
         raise RuntimeError(f"{name} must be a {cache.dtype} tensor on {cache.device}")
-    if t.numel() and (t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16):
+    st, sh, sd = t.stride()
+    if (sd != 1 or st % 8 or sh % 8 or t.data_ptr() % 16) and t.numel():
         raise RuntimeError(f"{name} needs unit stride in its last dimension, other strides a multiple of 8 and "
                            "16-byte alignment")
 
@@ -462,12 +473,10 @@ def kv4_append(cache: PagedKV4, q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
         if t.dtype not in (cache.dtype, torch.float32) or t.dtype != cos.dtype or t.device != dev:
             raise RuntimeError(f"cos and sin must both be {cache.dtype} or both float32, on {dev}")
     batch = _kv4_batch(cache, page_table, q_start, lengths)
-    with torch.cuda.device(dev):
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        rc = _lib.load().dscq_kv4_append(batch, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
-                                         k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), T, q.shape[1],
-                                         cos.data_ptr(), sin.data_ptr(), _DT[cos.dtype], cos.shape[0],
-                                         out.data_ptr(), _stream(dev))
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    rc = _launch(dev, _lib.load().dscq_kv4_append, batch, q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2],
+                 v.data_ptr(), *v.stride()[:2], T, q.shape[1], cos.data_ptr(), sin.data_ptr(), _DT[cos.dtype],
+                 cos.shape[0], out.data_ptr())
     _lib.check(rc, "kv4_append")
     return out
 
@@ -479,12 +488,22 @@ def kv4_read(cache: PagedKV4, page_table: torch.Tensor, q_start: torch.Tensor, l
     each sequence it reads whole sequences back."""
     dev = cache.device
     batch = _kv4_batch(cache, page_table, q_start, lengths)
-    with torch.cuda.device(dev):
-        k = torch.empty((rows, cache.kv_heads, cache.head_dim), dtype=cache.dtype, device=dev)
-        v = torch.empty_like(k)
-        rc = _lib.load().dscq_kv4_read(batch, rows, k.data_ptr(), v.data_ptr(), _stream(dev))
+    k = torch.empty((rows, cache.kv_heads, cache.head_dim), dtype=cache.dtype, device=dev)
+    v = torch.empty_like(k)
+    rc = _launch(dev, _lib.load().dscq_kv4_read, batch, rows, k.data_ptr(), v.data_ptr())
     _lib.check(rc, "kv4_read")
     return k, v
+
+
+_kv4_space: dict = {}
+
+
+def _kv4_workspace(dev: torch.device, head_dim: int) -> int:
+    key = (dev.index, head_dim)
+    if key not in _kv4_space:
+        with torch.cuda.device(dev):
+            _kv4_space[key] = _lib.load().dscq_kv4_attention_workspace(head_dim)
+    return _kv4_space[key]
 
 
 def kv4_attention(cache: PagedKV4, q: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor,
@@ -505,13 +524,11 @@ def kv4_attention(cache: PagedKV4, q: torch.Tensor, page_table: torch.Tensor, q_
     if max_q is not None and max_q < 0:
         raise RuntimeError("max_q must not be negative")
     batch = _kv4_batch(cache, page_table, q_start, lengths)
-    with torch.cuda.device(dev):
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        lib = _lib.load()
-        space = torch.empty(lib.dscq_kv4_attention_workspace(cache.head_dim), dtype=torch.uint8, device=dev)
-        rc = lib.dscq_kv4_attention(batch, q.data_ptr(), q.stride(0), q.stride(1), T, q.shape[1], max_q or 0,
-                                    cache.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(),
-                                    space.data_ptr(), space.numel(), _stream(dev))
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    size = _kv4_workspace(dev, cache.head_dim)
+    space = torch.empty(size, dtype=torch.uint8, device=dev)  # this call's own: calls may overlap, graphs keep theirs
+    rc = _launch(dev, _lib.load().dscq_kv4_attention, batch, q.data_ptr(), *q.stride()[:2], T, q.shape[1], max_q or 0,
+                 cache.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(), space.data_ptr(), size)
     _lib.check(rc, "kv4_attention")
     return out
 
@@ -543,13 +560,12 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) 
         raise RuntimeError("need 0 <= top_k <= 64 and top_k <= V")
     _no_grad_inputs(logits)
     dev = logits.device
-    with torch.cuda.device(dev):
-        stats = torch.empty((2, rows), dtype=torch.float32, device=dev)
-        top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
-        ids = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
-        rc = _lib.load().dscq_token_logprobs(logits.data_ptr(), _DT[logits.dtype], rows, V,
-                                             logits.stride(0) if rows > 1 else V, targets.data_ptr(), top_k,
-                                             stats[0].data_ptr(), stats[1].data_ptr(), top.data_ptr(),
-                                             ids.data_ptr(), _stream(dev))
+    stats = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+    ids = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
+    at = stats.data_ptr()
+    rc = _launch(dev, _lib.load().dscq_token_logprobs, logits.data_ptr(), _DT[logits.dtype], rows, V,
+                 logits.stride(0) if rows > 1 else V, targets.data_ptr(), top_k, at, at + 4 * rows, top.data_ptr(),
+                 ids.data_ptr())
     _lib.check(rc, "token_logprobs")
-    return TokenLogprobs(stats[0], stats[1], top, ids)
+    return TokenLogprobs(*stats.unbind(0), top, ids)
