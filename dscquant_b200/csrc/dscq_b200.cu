@@ -31,6 +31,7 @@
 #include "kv4.cuh"
 #include "kv4_attention.cuh"
 #include "kv4_decode.cuh"
+#include "kv4_prompt.cuh"
 #include "token_logprobs.cuh"
 
 namespace {
@@ -550,7 +551,22 @@ cudaError_t launch_kv4_decode(const dscq::Kv4AttnParams& a, int64_t max_rows, vo
 template <typename T, int D>
 cudaError_t launch_kv4_attention(const dscq::Kv4AttnParams& a, int64_t max_q, void* ws, cudaStream_t st) {
   const int64_t all = std::numeric_limits<int64_t>::max();
-  return max_q * a.group <= 8 ? launch_kv4_decode<T, D, 1>(a, all, ws, st) : launch_kv4_decode<T, D, 2>(a, all, ws, st);
+  const int64_t rows = max_q * a.group;
+  if (rows <= 8) return launch_kv4_decode<T, D, 1>(a, all, ws, st);
+  // Sequences of more than 64 rows go to the tensor-core kernel, when there can be enough of them to fill
+  // a quarter of the GPU with CTAs of 256 rows.
+  const int64_t few = 64;
+  const int64_t ctas = (static_cast<int64_t>(a.T) * a.group / 256 + std::min<int64_t>(a.b.B, a.T)) * a.b.hk;
+  if (rows <= few || (static_cast<int64_t>(a.T) * a.group + 255) / 256 * a.b.hk < num_sms() / 4 || ctas >= (int64_t(1) << 31))
+    return launch_kv4_decode<T, D, 2>(a, all, ws, st);
+  cudaError_t e = launch_kv4_decode<T, D, 2>(a, few, ws, st);
+  if (e != cudaSuccess) return e;
+  const dscq::Kv4PromptParams p{a, few + 1};
+  constexpr int smem = dscq::Kv4PromptConfig<D>::kSmem;
+  e = cudaFuncSetAttribute(dscq::kv4_prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  dscq::kv4_prompt_kernel<T, D><<<static_cast<unsigned>(ctas), dscq::kKv4PromptThreads, smem, st>>>(p);
+  return cudaGetLastError();
 }
 
 // f.template operator()<T, D>() for the cache's type and head dimension.

@@ -1,0 +1,442 @@
+// Attention of many rows per sequence (prompts and their chunks) over the 4-bit paged cache: bound by the tensor cores
+// and the exponentials. See kv4_attention.cuh for the operator.
+//
+// A CTA takes 256 rows (tokens x query heads of one key head) of a sequence as two tiles of 128 and runs over the
+// keys they see, 128 at a time, with tcgen05 (kind::f16, M = 128):
+//   S_i = Q_i K^T   (TMEM, 128 columns each)     P_i = exp2(S_i - max) over S_i     O_i += P_i V   (TMEM)
+// While one tile's softmax runs, the other's products do. TMEM: S_0/P_0, S_1/P_1, O_0, O_1 = 512 columns.
+//
+// Operands are fp16 whatever the cache's type. Codes become numbers on the way into shared memory, four warps, one key
+// a thread: a code in the low bits of an fp16 is the subnormal n 2^-24, so an AND and a fused multiply-add give
+// round(n step' + low') for two elements, with (step', low') scaled by a power of two that puts the tile's largest
+// value under 2^-6 (for values: the largest so far; sums already made follow). That rounds keys and values to 11
+// bits; queries, scaled by a power of two a row, are exact. Scores, statistics and sums are 32-bit. Weights are
+// fp16, relative to a running maximum that only moves when it would be passed by 2^8: then the row's sums in
+// TMEM are scaled, by the warps that own them.
+//
+// Keys no row may see (behind the end, on pages out of range) are zeros with their scores masked. A value row that is
+// not finite is zeros too and flagged; rows that see its key become NaN, the others must not.
+//
+// Warps 0-3, 4-7: softmax of tile 0 and 1 (a thread a row); 8-11: codes to operands; 12: MMA. All waits bounded.
+#pragma once
+#include "kv4_decode.cuh"
+
+namespace dscq {
+
+struct Kv4PromptParams {
+  Kv4AttnParams a;
+  int64_t min_rows;  // sequences with fewer rows * group than this are not this kernel's
+};
+
+constexpr int kKv4PromptThreads = 13 * 32;
+constexpr int64_t kKv4AllRows = INT64_MAX;
+
+// x 2^e in two steps, for |e| up to 250.
+__device__ __forceinline__ float times_pow2(float x, int e) { return x * pow2f(e / 2) * pow2f(e - e / 2); }
+
+// kind::f16 with fp16 A and B, f32 D; A K-major, B K-major or MN-major (bit 16).
+__host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n, bool b_mn) {
+  return (1u << 4) | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+// D[tmem] (+)= A[tmem] B[smem], A: a lane a row, two consecutive k a column.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+template <int D>
+struct Kv4PromptConfig {
+  static constexpr int kHalf = 128 * 128;               // 128 rows of 64 fp16, 128-byte swizzled
+  static constexpr int kTile = D / 64 * kHalf;          // an operand of 128 rows
+  static constexpr int kSmem = 1024 + 6 * kTile + 1024; // Q_0, Q_1, two stages of K and of V; barriers, tile facts
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const Kv4PromptParams p) {
+  using C = Kv4PromptConfig<D>;
+  const Kv4AttnParams& a = p.a;
+  extern __shared__ uint8_t kv4_prompt_smem[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kv4_prompt_smem) + 1023) & ~uintptr_t(1023));
+  uint8_t* qs = smem;                  // [2]
+  uint8_t* ks = smem + 2 * C::kTile;   // [2]
+  uint8_t* vs = smem + 4 * C::kTile;   // [2]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 6 * C::kTile);
+  uint64_t *qfull = bars, *kfull = bars + 1, *kempty = bars + 3, *vfull = bars + 5, *vempty = bars + 7;
+  uint64_t *sfull = bars + 9, *pfull = bars + 11, *ofull = bars + 13, *done = bars + 15;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* item = reinterpret_cast<int*>(tmem_slot + 2);       // sequence, head, row tile
+  int* kexp = item + 4;                                    // [2] exponents of the stages' scales
+  int* vexp = kexp + 2;
+  uint32_t* hide = reinterpret_cast<uint32_t*>(vexp + 2);  // [2][4] keys on pages out of range
+  uint32_t* poison = hide + 8;                             // [2][4] keys whose values are not finite
+  float* tile_max = reinterpret_cast<float*>(poison + 8);  // [2][4][2]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (warp == 12) {
+    // this CTA's 256 rows; of a sequence the last ones, which see the most keys, first
+    int64_t left = blockIdx.x;
+    int seq = -1, head = 0, tile = 0;
+    for (int s0 = 0; s0 < a.b.B && seq < 0; s0 += 32) {
+      const int s = s0 + lane;
+      int64_t tiles = 0;
+      if (s < a.b.B) {
+        const Kv4Seq r = kv4_seq<128, 256>(a, kKv4AllRows, s);
+        tiles = static_cast<int64_t>(r.n) * a.group < p.min_rows ? 0 : r.blocks;
+      }
+      int64_t upto = tiles * a.b.hk;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, upto > left);
+      if (past) {
+        const int src = __ffs(past) - 1;
+        seq = s0 + src;
+        const int n = static_cast<int>(__shfl_sync(0xffffffffu, tiles, src));
+        const int at = static_cast<int>(left - __shfl_sync(0xffffffffu, upto - tiles * a.b.hk, src));
+        tile = n - 1 - at / a.b.hk;
+        head = at % a.b.hk;
+      } else {
+        left -= __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+    if (lane == 0) {
+      item[0] = seq, item[1] = head, item[2] = tile;
+      mbar_init(qfull, 8);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(kfull + i, 4);
+        mbar_init(vfull + i, 4);
+        mbar_init(kempty + i, 1);
+        mbar_init(vempty + i, 1);
+        mbar_init(sfull + i, 1);
+        mbar_init(pfull + i, 4);
+        mbar_init(ofull + i, 1);
+      }
+      mbar_init(done, 1);
+      *abort_flag = 0;
+      fence_mbar_init();
+    }
+    __syncwarp();
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int seq = item[0], head = item[1], r0 = item[2] * 256;
+  if (seq >= 0) {
+    const Kv4Seq sq = kv4_seq<128, 256>(a, kKv4AllRows, seq);
+    const int rows = sq.n * a.group;
+    const int halves = r0 + 128 < rows ? 2 : 1;
+    // keys of row r: positions up to its own
+    auto limit = [&](int r) { return min(sq.keys, sq.len - sq.n + a.row_token(r) + 1); };
+    const int tiles = max((limit(min(r0 + 256, rows) - 1) + 127) / 128, 1);
+
+    if (warp < 8) {
+      // ------------------------------------------------ queries, softmax, output: a thread a row
+      const int half = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + half * 128 + row;
+      const bool live = half < halves, real = live && r < rows;
+      const int tok = a.row_token(real ? r : 0);
+      const int64_t hd = head * a.group + (real ? r - tok * a.group : 0);
+      float c1 = 0.f;
+      if (live) {
+        uint4 x[D / 8];
+        float big = 0.f;
+        const T* src = static_cast<const T*>(a.q) + (sq.q0 + static_cast<int64_t>(tok)) * a.q_t + hd * a.q_h;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          x[c] = real ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
+          float f[8];
+          kv4_unpack8<T>(x[c], f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(f[e]));
+        }
+        // as in kv4_decode.cuh: the row's largest element in [2^14, 2^15), a negative scale turns the queries around
+        const int k = big > 0.f && big < INFINITY ? min(max(14 - log2i(big), -90), 120) : 0;
+        const float f = a.scale_log2 == 0.f ? 0.f : copysignf(pow2f(k), a.scale_log2);
+        c1 = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2) * pow2f(-k);
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          float y[8];
+          kv4_unpack8<T>(x[c], y);
+          // element order 0 4 1 5 2 6 3 7, as the codes come apart
+          const uint4 o = make_uint4(pack2<__half>(y[0] * f, y[4] * f), pack2<__half>(y[1] * f, y[5] * f),
+                                     pack2<__half>(y[2] * f, y[6] * f), pack2<__half>(y[3] * f, y[7] * f));
+          *reinterpret_cast<uint4*>(qs + half * C::kTile + (c >> 3) * C::kHalf + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = o;
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(qfull);
+
+      if (live) {
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_at = tmem + half * 128 + lanes, o_at = tmem + 256 + half * 128 + lanes;
+        const int lim = real ? limit(r) : 0;
+        float m = -INFINITY, l[4] = {0.f, 0.f, 0.f, 0.f};
+        int ev = -200;
+        bool ok = true, nan = false;
+        for (int t = 0; t < tiles; ++t) {
+          const int s = t & 1;
+          const uint32_t ph = (t >> 1) & 1u;
+          ok = mbar_wait(&sfull[half], t & 1u, abort_flag) && mbar_wait(&vfull[s], ph, abort_flag);
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const int see = lim - t * 128;  // columns this row sees
+          const uint32_t hidden = hide[s * 4] | hide[s * 4 + 1] | hide[s * 4 + 2] | hide[s * 4 + 3];
+          const uint32_t bad = poison[s * 4] | poison[s * 4 + 1] | poison[s * 4 + 2] | poison[s * 4 + 3];
+          const bool masked = __any_sync(0xffffffffu, see < 128) || hidden;
+          if (bad) {
+            for (int j = 0; j < min(see, 128); ++j)
+              if ((poison[s * 4 + (j >> 5)] & ~hide[s * 4 + (j >> 5)]) >> (j & 31) & 1u) nan = true;
+          }
+          auto mask = [&](uint32_t (&v)[32], int c) {
+            const uint32_t h = hide[s * 4 + c];
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c * 32 + j >= see || (h >> j & 1u)) v[j] = 0xff800000u;
+          };
+          // ---- the tile's maximum
+          float mt = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32];
+            tmem_ld32(s_at + c * 32, v);
+            tmem_ld_wait();
+            if (masked) mask(v, c);
+#pragma unroll
+            for (int j = 0; j < 32; j += 2)
+              mt = fmaxf(fmaxf(mt, __uint_as_float(v[j])), __uint_as_float(v[j + 1]));
+          }
+          const float ce = times_pow2(c1, kexp[s]);
+          mt = mt == -INFINITY ? mt : mt * ce;
+          float f = 1.f;
+          if (mt > m + 8.f || (m == -INFINITY && mt > m)) {
+            f = ex2(m - mt);
+            m = mt;
+          }
+          const int e = vexp[s];
+          const float fo = e == ev ? f : f * pow2f(max(ev - e, -126));  // e never falls
+          ev = e;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) l[j] *= f;
+          if (t > 0 && __any_sync(0xffffffffu, fo != 1.f)) {
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              uint32_t v[32];
+              tmem_ld32(o_at + c, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * fo);
+              tmem_st16(o_at + c, reinterpret_cast<const uint32_t(&)[16]>(v[0]));
+              tmem_st16(o_at + c + 16, reinterpret_cast<const uint32_t(&)[16]>(v[16]));
+            }
+          }
+          // ---- weights, over the scores they come from
+          const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32], w[16];
+            tmem_ld32(s_at + c * 32, v);
+            tmem_ld_wait();
+            if (masked) mask(v, c);
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const float p0 = ex2(fmaf(__uint_as_float(v[j]), ce, -base)), p1 = ex2(fmaf(__uint_as_float(v[j + 1]), ce, -base));
+              l[j & 2] += p0;
+              l[(j & 2) + 1] += p1;
+              w[j / 2] = pack2<__half>(p0, p1);
+            }
+            tmem_st16(s_at + c * 16, w);
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pfull[half]);
+        }
+        ok = ok && mbar_wait(&ofull[half], 0, abort_flag);
+        if (__all_sync(0xffffffffu, ok)) {
+          tc_fence_after();
+          const float sum = (l[0] + l[1]) + (l[2] + l[3]);
+          const float inv = nan ? __int_as_float(0x7fc00000) : sum == 0.f ? 0.f : 1.f / sum;
+          T* out = static_cast<T*>(a.out) + ((sq.q0 + static_cast<int64_t>(tok)) * a.hq + hd) * D;
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            uint32_t v[32];
+            tmem_ld32(o_at + c, v);
+            tmem_ld_wait();
+            if (real) {
+#pragma unroll
+              for (int j = 0; j < 32; j += 8) {
+                float y[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = times_pow2(__uint_as_float(v[j + i]) * inv, ev);
+                *reinterpret_cast<uint4*>(out + c + j) = make_uint4(pack2<T>(y[0], y[2]), pack2<T>(y[4], y[6]),
+                                                                    pack2<T>(y[1], y[3]), pack2<T>(y[5], y[7]));
+              }
+            }
+          }
+        }
+      }
+    } else if (warp < 12) {
+      // ------------------------------------------------ codes to operands: a thread a key
+      const int key = threadIdx.x - 256, part = warp - 8;
+      uint4 kc[D / 32], vc[D / 32];
+      uint32_t ka = 0, va = 0;
+      bool have = false, lost = false;
+      int page = -1;
+      auto look = [&](int t) {  // the page of this thread's key in tile t; -1 behind the end
+        const int at = t * 128 + key;
+        page = t < tiles && at < sq.keys ? a.b.table[seq * a.b.ld_table + (at >> a.b.ps_log2)] : -1;
+      };
+      auto row_of = [&](int t) {
+        return ((static_cast<int64_t>(page) * a.b.hk + head) << a.b.ps_log2) + ((t * 128 + key) & ((1 << a.b.ps_log2) - 1));
+      };
+      auto load = [&](int t) {
+        have = page >= 0 && page < a.b.pages;
+        lost = !have && t < tiles && t * 128 + key < sq.keys;
+        ka = va = 0;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) kc[c] = vc[c] = make_uint4(0, 0, 0, 0);
+        if (!have) return;
+        const int64_t row = row_of(t);
+        ka = a.b.ka[row];
+        va = a.b.va[row];
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          kc[c] = reinterpret_cast<const uint4*>(a.b.kc + row * (D / 2))[c];
+          vc[c] = reinterpret_cast<const uint4*>(a.b.vc + row * (D / 2))[c];
+        }
+      };
+      // (step 2^24, step 2^20, low) under a scale of 2^-x as pairs of fp16
+      auto expand = [&](uint8_t* dst, const uint4 (&codes)[D / 32], float2 f, int x) {
+        const float st = times_pow2(f.x, -x), lo = times_pow2(f.y, -x);
+        const __half2 s24 = __float2half2_rn(st * 0x1p24f), s20 = __float2half2_rn(st * 0x1p20f), l2 = __float2half2_rn(lo);
+        auto two = [&](uint32_t w, const __half2& by) {
+          __half2 h;
+          memcpy(&h, &w, 4);
+          h = __hfma2(h, by, l2);
+          memcpy(&w, &h, 4);
+          return w;
+        };
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 q4 = codes[c / 4];
+          const uint32_t w = c % 4 == 0 ? q4.x : c % 4 == 1 ? q4.y : c % 4 == 2 ? q4.z : q4.w, u = w >> 8;
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * C::kHalf + key * 128 + (((c & 7) ^ (key & 7)) << 4)) =
+              make_uint4(two(w & kCode0, s24), two(w & kCode1, s20), two(u & kCode0, s24), two(u & kCode1, s20));
+        }
+      };
+      look(0);
+      load(0);
+      look(1);
+      int run = -100;  // exponent of the largest value so far
+      for (int t = 0; t < tiles; ++t) {
+        const int s = t & 1;
+        const uint32_t ph = (t >> 1) & 1u;
+        float2 kf = unpack2<T>(ka), vf = unpack2<T>(va);
+        const bool sick = !isfinite(vf.x) || !isfinite(vf.y);
+        if (sick) vf = make_float2(0.f, 0.f);
+        float km = fmaxf(fabsf(kf.y), fabsf(fmaf(15.f, kf.x, kf.y)));
+        float vm = fmaxf(fabsf(vf.y), fabsf(fmaf(15.f, vf.x, vf.y)));
+        if (!(km < INFINITY)) km = 0.f;
+        if (!(vm < INFINITY)) vm = 0x1.fffffep127f;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+          km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, o));
+          vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
+        }
+        if (lane == 0) tile_max[(s * 4 + part) * 2] = km, tile_max[(s * 4 + part) * 2 + 1] = vm;
+        const unsigned gone = __ballot_sync(0xffffffffu, lost), ill = __ballot_sync(0xffffffffu, sick && have);
+        named_bar_sync(1, 128);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          km = fmaxf(km, tile_max[(s * 4 + i) * 2]);
+          vm = fmaxf(vm, tile_max[(s * 4 + i) * 2 + 1]);
+        }
+        const int kx = max(log2i(km), -100) + 7;  // the largest goes under 2^-6
+        run = max(run, log2i(vm) + 7);
+        if (lost) raise_status(kStatusBadIndex);
+
+        bool ok = t < 2 || mbar_wait(&kempty[s], ph ^ 1u, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        expand(ks + s * C::kTile, kc, kf, kx);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&kfull[s]);
+        ok = t < 2 || mbar_wait(&vempty[s], ph ^ 1u, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        expand(vs + s * C::kTile, vc, vf, run);
+        if (lane == 0) {  // the tile's facts: its stage's last user read them before its values were multiplied
+          hide[s * 4 + part] = gone;
+          poison[s * 4 + part] = ill;
+          if (part == 0) kexp[s] = kx, vexp[s] = run;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&vfull[s]);
+        load(t + 1);
+        look(t + 2);
+      }
+    } else if (lane == 0) {
+      // ------------------------------------------------ MMA
+      constexpr uint32_t id_qk = umma_idesc_f16(128, 128, false), id_pv = umma_idesc_f16(128, D, true);
+      auto scores = [&](int i, int s) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = static_cast<uint32_t>((k >> 2) * C::kHalf + (k & 3) * 32);
+          umma_f16_ss(tmem + i * 128, umma_desc_sw128(smem_u32(qs + i * C::kTile) + off),
+                      umma_desc_sw128(smem_u32(ks + s * C::kTile) + off), id_qk, k > 0 ? 1u : 0u);
+        }
+        umma_commit(&sfull[i]);
+        if (i + 1 == halves) umma_commit(&kempty[s]);
+      };
+      bool ok = mbar_wait(qfull, 0, abort_flag) && mbar_wait(&kfull[0], 0, abort_flag);
+      tc_fence_after();
+      for (int i = 0; ok && i < halves; ++i) scores(i, 0);
+      for (int t = 0; ok && t < tiles; ++t) {
+        const int s = t & 1;
+        for (int i = 0; ok && i < halves; ++i) {
+          if (i == 0) ok = mbar_wait(&vfull[s], (t >> 1) & 1u, abort_flag);
+          ok = ok && mbar_wait(&pfull[i], t & 1u, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + k * 8,
+                        umma_desc_sw128_mn_atoms(smem_u32(vs + s * C::kTile) + k * 2048, C::kHalf), id_pv,
+                        t > 0 || k > 0 ? 1u : 0u);
+          if (i + 1 == halves) umma_commit(&vempty[s]);
+          if (t + 1 == tiles) {
+            umma_commit(&ofull[i]);
+          } else {
+            if (i == 0) ok = mbar_wait(&kfull[s ^ 1], ((t + 1) >> 1) & 1u, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            scores(i, s ^ 1);
+          }
+        }
+      }
+      umma_commit(done);
+      mbar_wait(done, 0, nullptr);  // nothing is in flight when the memory goes
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  __syncthreads();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace dscq

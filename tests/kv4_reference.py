@@ -92,8 +92,10 @@ class Batch:
         return slice(self.starts[b], self.starts[b + 1]), range(L - n, L)
 
     def attention(self, q, scale=None):
-        """(out, bound) in float64. `bound`: how far a kernel may be off before its last rounding, when it
-        keeps scores and sums in 32 bits and rounds each softmax weight to 16 bits once."""
+        """(out, bound) in float64. `bound`: how far a kernel may be off before its last rounding, when it keeps
+        scores and sums in 32 bits, rounds each softmax weight to the cache's type or better once, and may
+        take keys, values and weights as fp16 scaled by powers of two (11 bits, 2^-18 of the largest at least,
+        weights 2^-25 at least)."""
         T, hq, D = q.shape
         group = hq // self.kv_heads
         scale = D ** -0.5 if scale is None else scale
@@ -117,9 +119,12 @@ class Batch:
                     p = torch.where(seen.any(-1, keepdim=True), p, 0.0)
                     out[rows, g] = p @ v
                     # scores: D products of |q| times up to 32 steps (codes as 16..31 sixteenths) and the low
-                    # part, each accumulation off by 2^-23; weights follow as exp of that error, on both sides
-                    # of the normalisation; the exponential and the sums add 2^-20
+                    # part, each accumulation off by 2^-23, and keys rounded to 11 bits; weights follow as exp of
+                    # that error, on both sides of the normalisation; the exponential and the sums add 2^-20
                     size = x.abs().sum(-1, keepdim=True) * (32 * ka[:, 0].abs().max() + ka[:, 1].abs().max())
-                    off_s = 2.0 ** -23 * D * abs(scale) * size + 2.0 ** -20
-                    bound[rows, g] = half * 1.01 * (p @ (v - va[:, 1:]).abs()) + 2.1 * off_s * (p @ v.abs())
+                    rounded = torch.where(seen, x.abs() @ k.abs().T, 0.0).amax(-1, keepdim=True) * 2.0 ** -12 + \
+                        x.abs().sum(-1, keepdim=True) * k.abs().max() * 2.0 ** -18
+                    off_s = abs(scale) * (2.0 ** -23 * D * size + rounded) + 2.0 ** -20
+                    bound[rows, g] = half * 1.01 * (p @ (v - va[:, 1:]).abs()) + 2.1 * off_s * (p @ v.abs()) + \
+                        2.0 ** -11 * (p @ v.abs()) + (2.0 ** -18 + L * 2.0 ** -25) * v.abs().max()
         return out, bound
