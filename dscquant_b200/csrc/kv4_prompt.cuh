@@ -50,6 +50,16 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       : "memory");
 }
 
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(is));
+  return is != 0;
+}
+
 template <int D>
 struct Kv4PromptConfig {
   static constexpr int kHalf = 128 * 128;               // 128 rows of 64 fp16, 128-byte swizzled
@@ -68,8 +78,8 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
   uint8_t* vs = smem + 4 * C::kTile;   // [2]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 6 * C::kTile);
   uint64_t *qfull = bars, *kfull = bars + 1, *kempty = bars + 3, *vfull = bars + 5, *vempty = bars + 7;
-  uint64_t *sfull = bars + 9, *pfull = bars + 11, *ofull = bars + 13, *done = bars + 15;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+  uint64_t *sfull = bars + 9, *pfull = bars + 11, *ofull = bars + 15, *done = bars + 17;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* item = reinterpret_cast<int*>(tmem_slot + 2);       // sequence, head, row tile
   int* kexp = item + 4;                                    // [2] exponents of the stages' scales
@@ -117,7 +127,8 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
         mbar_init(kempty + i, 1);
         mbar_init(vempty + i, 1);
         mbar_init(sfull + i, 1);
-        mbar_init(pfull + i, 4);
+        mbar_init(pfull + 2 * i, 4);
+        mbar_init(pfull + 2 * i + 1, 4);
         mbar_init(ofull + i, 1);
       }
       mbar_init(done, 1);
@@ -181,29 +192,30 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
       if (live) {
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + half * 128 + lanes, o_at = tmem + 256 + half * 128 + lanes;
-        const int lim = real ? limit(r) : 0;
+        const int lim = real ? limit(r) : INT_MAX;  // a row of nothing masks nothing
         float m = -INFINITY, l[4] = {0.f, 0.f, 0.f, 0.f};
         int ev = -200;
         bool ok = true, nan = false;
         for (int t = 0; t < tiles; ++t) {
           const int s = t & 1;
           const uint32_t ph = (t >> 1) & 1u;
-          ok = mbar_wait(&sfull[half], t & 1u, abort_flag) && mbar_wait(&vfull[s], ph, abort_flag);
+          ok = mbar_wait_spin(&sfull[half], t & 1u, abort_flag) && mbar_wait_spin(&vfull[s], ph, abort_flag);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const int see = lim - t * 128;  // columns this row sees
+          const int see = min(lim - t * 128, 128);  // columns this row sees
           const uint32_t hidden = hide[s * 4] | hide[s * 4 + 1] | hide[s * 4 + 2] | hide[s * 4 + 3];
           const uint32_t bad = poison[s * 4] | poison[s * 4 + 1] | poison[s * 4 + 2] | poison[s * 4 + 3];
           const bool masked = __any_sync(0xffffffffu, see < 128) || hidden;
           if (bad) {
-            for (int j = 0; j < min(see, 128); ++j)
+            for (int j = 0; j < see; ++j)
               if ((poison[s * 4 + (j >> 5)] & ~hide[s * 4 + (j >> 5)]) >> (j & 31) & 1u) nan = true;
           }
           auto mask = [&](uint32_t (&v)[32], int c) {
             const uint32_t h = hide[s * 4 + c];
+            if (!__any_sync(0xffffffffu, see < (c + 1) * 32 || h)) return;
 #pragma unroll
             for (int j = 0; j < 32; ++j)
               if (c * 32 + j >= see || (h >> j & 1u)) v[j] = 0xff800000u;
@@ -246,27 +258,32 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
           }
           // ---- weights, over the scores they come from
           const float base = m == -INFINITY ? 0.f : m;
+          uint32_t v[2][32];
+          tmem_ld32(s_at, v[0]);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            uint32_t v[32], w[16];
-            tmem_ld32(s_at + c * 32, v);
             tmem_ld_wait();
-            if (masked) mask(v, c);
+            if (c < 3) tmem_ld32(s_at + (c + 1) * 32, v[(c + 1) & 1]);
+            if (masked) mask(v[c & 1], c);
+            uint32_t w[16];
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
-              const float p0 = ex2(fmaf(__uint_as_float(v[j]), ce, -base)), p1 = ex2(fmaf(__uint_as_float(v[j + 1]), ce, -base));
+              const float p0 = ex2(fmaf(__uint_as_float(v[c & 1][j]), ce, -base));
+              const float p1 = ex2(fmaf(__uint_as_float(v[c & 1][j + 1]), ce, -base));
               l[j & 2] += p0;
               l[(j & 2) + 1] += p1;
               w[j / 2] = pack2<__half>(p0, p1);
             }
             tmem_st16(s_at + c * 16, w);
+            if (c & 1) {
+              tmem_st_wait();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&pfull[2 * half + (c >> 1)]);
+            }
           }
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&pfull[half]);
         }
-        ok = ok && mbar_wait(&ofull[half], 0, abort_flag);
+        ok = ok && mbar_wait_spin(&ofull[half], 0, abort_flag);
         if (__all_sync(0xffffffffu, ok)) {
           tc_fence_after();
           const float sum = (l[0] + l[1]) + (l[2] + l[3]);
@@ -370,13 +387,13 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
         run = max(run, log2i(vm) + 7);
         if (lost) raise_status(kStatusBadIndex);
 
-        bool ok = t < 2 || mbar_wait(&kempty[s], ph ^ 1u, abort_flag);
+        bool ok = t < 2 || mbar_wait_spin(&kempty[s], ph ^ 1u, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) break;
         expand(ks + s * C::kTile, kc, kf, kx);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&kfull[s]);
-        ok = t < 2 || mbar_wait(&vempty[s], ph ^ 1u, abort_flag);
+        ok = t < 2 || mbar_wait_spin(&vempty[s], ph ^ 1u, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) break;
         expand(vs + s * C::kTile, vc, vf, run);
         if (lane == 0) {  // the tile's facts: its stage's last user read them before its values were multiplied
@@ -390,47 +407,59 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
         load(t + 1);
         look(t + 2);
       }
-    } else if (lane == 0) {
-      // ------------------------------------------------ MMA
+    } else {
+      // ------------------------------------------------ MMA: the warp walks together, so addresses stay uniform
       constexpr uint32_t id_qk = umma_idesc_f16(128, 128, false), id_pv = umma_idesc_f16(128, D, true);
+      const uint64_t q_desc = umma_desc_sw128(smem_u32(qs)), k_desc = umma_desc_sw128(smem_u32(ks));
+      const uint64_t v_desc = umma_desc_sw128_mn_atoms(smem_u32(vs), C::kHalf);
       auto scores = [&](int i, int s) {
+        const uint64_t qd = q_desc + static_cast<uint32_t>(i * C::kTile >> 4), kd = k_desc + static_cast<uint32_t>(s * C::kTile >> 4);
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = static_cast<uint32_t>((k >> 2) * C::kHalf + (k & 3) * 32);
-          umma_f16_ss(tmem + i * 128, umma_desc_sw128(smem_u32(qs + i * C::kTile) + off),
-                      umma_desc_sw128(smem_u32(ks + s * C::kTile) + off), id_qk, k > 0 ? 1u : 0u);
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t off = static_cast<uint32_t>((k >> 2) * C::kHalf + (k & 3) * 32) >> 4;
+            umma_f16_ss(tmem + i * 128, qd + off, kd + off, id_qk, k > 0 ? 1u : 0u);
+          }
+          umma_commit(&sfull[i]);
+          if (i + 1 == halves) umma_commit(&kempty[s]);
         }
-        umma_commit(&sfull[i]);
-        if (i + 1 == halves) umma_commit(&kempty[s]);
+        __syncwarp();
       };
-      bool ok = mbar_wait(qfull, 0, abort_flag) && mbar_wait(&kfull[0], 0, abort_flag);
+      bool ok = mbar_wait_spin(qfull, 0, abort_flag) && mbar_wait_spin(&kfull[0], 0, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
       for (int i = 0; ok && i < halves; ++i) scores(i, 0);
       for (int t = 0; ok && t < tiles; ++t) {
         const int s = t & 1;
+        const uint64_t vd = v_desc + static_cast<uint32_t>(s * C::kTile >> 4);
         for (int i = 0; ok && i < halves; ++i) {
-          if (i == 0) ok = mbar_wait(&vfull[s], (t >> 1) & 1u, abort_flag);
-          ok = ok && mbar_wait(&pfull[i], t & 1u, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
+          if (i == 0) ok = mbar_wait_spin(&vfull[s], (t >> 1) & 1u, abort_flag);
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + k * 8,
-                        umma_desc_sw128_mn_atoms(smem_u32(vs + s * C::kTile) + k * 2048, C::kHalf), id_pv,
-                        t > 0 || k > 0 ? 1u : 0u);
-          if (i + 1 == halves) umma_commit(&vempty[s]);
-          if (t + 1 == tiles) {
-            umma_commit(&ofull[i]);
-          } else {
-            if (i == 0) ok = mbar_wait(&kfull[s ^ 1], ((t + 1) >> 1) & 1u, abort_flag);
+          for (int part = 0; part < 2; ++part) {  // weights of 64 keys at a time
+            ok = ok && mbar_wait_spin(&pfull[2 * i + part], t & 1u, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int k = 4 * part; k < 4 * part + 4; ++k)
+                umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + k * 8, vd + (k * 2048 >> 4), id_pv,
+                            t > 0 || k > 0 ? 1u : 0u);
+              if (part == 1 && i + 1 == halves) umma_commit(&vempty[s]);
+              if (part == 1 && t + 1 == tiles) umma_commit(&ofull[i]);
+            }
+            __syncwarp();
+          }
+          if (ok && t + 1 < tiles) {
+            if (i == 0) ok = __all_sync(0xffffffffu, mbar_wait_spin(&kfull[s ^ 1], ((t + 1) >> 1) & 1u, abort_flag));
             if (!ok) break;
             tc_fence_after();
             scores(i, s ^ 1);
           }
         }
       }
-      umma_commit(done);
-      mbar_wait(done, 0, nullptr);  // nothing is in flight when the memory goes
+      if (elect_one()) umma_commit(done);
+      mbar_wait_spin(done, 0, nullptr);  // nothing is in flight when the memory goes
     }
   }
   tc_fence_before();
