@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 NATIVE_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_native")
@@ -24,15 +25,8 @@ _i32, _i64, _u32p, _f32, _vp, _cp = (ctypes.c_int, ctypes.c_int64, ctypes.POINTE
                                      ctypes.c_void_p, ctypes.c_char_p)
 
 
-class Kv4Batch(ctypes.Structure):
-    """dscq_kv4_batch."""
-    _fields_ = [("k_codes", _vp), ("k_affine", _vp), ("v_codes", _vp), ("v_affine", _vp), ("pages", _i64),
-                ("kv_heads", ctypes.c_int32), ("page_size", ctypes.c_int32), ("head_dim", ctypes.c_int32),
-                ("dtype", ctypes.c_int32), ("page_table", _vp), ("ld_table", _i64), ("max_pages", _i64),
-                ("q_start", _vp), ("lengths", _vp), ("seqs", _i64)]
-
-
-_kv4p = ctypes.POINTER(Kv4Batch)
+# dscq_kv4_batch, passed as its bytes: packing them costs a fifth of filling a ctypes.Structure
+KV4_BATCH = struct.Struct("@PPPPqiiiiPqqPPq")
 
 # name -> (restype, argtypes); kept in the order of include/dscq_b200.h
 SIGNATURES = {
@@ -61,11 +55,11 @@ SIGNATURES = {
     "dscq_rmsnorm": (_i32, [_vp, _vp, _i64, _i64, _f32, _vp, _vp]),
     "dscq_rope": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp]),
     "dscq_silu_mul": (_i32, [_vp, _vp, _i64, _vp, _vp]),
-    "dscq_kv4_append": (_i32, [_kv4p, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _i32,
+    "dscq_kv4_append": (_i32, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _i32,
                                _i64, _vp, _vp]),
-    "dscq_kv4_read": (_i32, [_kv4p, _i64, _vp, _vp, _vp]),
+    "dscq_kv4_read": (_i32, [_vp, _i64, _vp, _vp, _vp]),
     "dscq_kv4_attention_workspace": (_i64, [_i32]),
-    "dscq_kv4_attention": (_i32, [_kv4p, _vp, _i64, _i64, _i64, _i32, _i64, _f32, _vp, _vp, _i64, _vp]),
+    "dscq_kv4_attention": (_i32, [_vp, _vp, _i64, _i64, _i64, _i32, _i64, _f32, _vp, _vp, _i64, _vp]),
     "dscq_token_logprobs": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _vp]),
     "dscq_pack_int4": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "dscq_unpack_int4": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp]),

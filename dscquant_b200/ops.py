@@ -415,38 +415,40 @@ def _no_grad_inputs(*tensors: torch.Tensor) -> None:
                 raise RuntimeError("this operator has no backward pass: call it under torch.no_grad()")
 
 
-def _kv4_batch(cache: PagedKV4, page_table: torch.Tensor, q_start: torch.Tensor, lengths: torch.Tensor):
+def _kv4_batch(cache: PagedKV4, page_table: torch.Tensor, q_start: torch.Tensor, lengths: torch.Tensor) -> bytes:
     """The dscq_kv4_batch of a call, after the checks every cache operator makes."""
-    dev = cache.device
-    if not (page_table.dtype == q_start.dtype == lengths.dtype == torch.int32 and
-            page_table.device == q_start.device == lengths.device == dev):
-        raise RuntimeError(f"page_table, q_start and lengths must be int32 tensors on {dev}")
+    i32, index = torch.int32, cache.index
+    if page_table.dtype is not i32 or q_start.dtype is not i32 or lengths.dtype is not i32 or \
+            page_table.get_device() != index or q_start.get_device() != index or lengths.get_device() != index:
+        raise RuntimeError(f"page_table, q_start and lengths must be int32 tensors on {cache.device}")
+    table = page_table.shape
     if lengths.dim() != 1 or q_start.shape != (lengths.shape[0] + 1,):
         raise RuntimeError("need lengths [B] and q_start [B + 1]")
     B = lengths.shape[0]
-    if page_table.dim() != 2 or page_table.shape[0] != B:
+    if len(table) != 2 or table[0] != B:
         raise RuntimeError("page_table must be [B, pages]")
-    P, ld = page_table.shape[1], page_table.stride(0)
-    if (P > 1 and page_table.stride(1) != 1) or (B and q_start.stride(0) != 1) or \
-            (B > 1 and (ld < P or lengths.stride(0) != 1)):
+    P = table[1]
+    ld, step = page_table.stride()
+    if (P > 1 and step != 1) or (B and q_start.stride(0) != 1) or (B > 1 and (ld < P or lengths.stride(0) != 1)):
         raise RuntimeError("page_table rows, q_start and lengths must be contiguous")
-    codes = cache.k_codes
-    pages, hk, ps, half = codes.shape
-    return _lib.Kv4Batch(codes.data_ptr(), cache.k_affine.data_ptr(), cache.v_codes.data_ptr(),
-                         cache.v_affine.data_ptr(), pages, hk, ps, half * 2, _DT[cache.dtype],
-                         page_table.data_ptr(), max(ld, P), P, q_start.data_ptr(), lengths.data_ptr(), B)
+    return _lib.KV4_BATCH.pack(cache.k_codes.data_ptr(), cache.k_affine.data_ptr(), cache.v_codes.data_ptr(),
+                               cache.v_affine.data_ptr(), cache.pages, cache.kv_heads, cache.page_size, cache.head_dim,
+                               cache.type_code, page_table.data_ptr(), max(ld, P), P, q_start.data_ptr(),
+                               lengths.data_ptr(), B)
 
 
-def _kv4_rows(cache: PagedKV4, name: str, t: torch.Tensor, T: int, heads: int | None) -> None:
-    shape = t.shape
-    if len(shape) != 3 or shape[0] != T or shape[2] != cache.head_dim or (heads is not None and shape[1] != heads):
-        raise RuntimeError(f"{name} must be [{T}, {heads or 'heads'}, {cache.head_dim}]")
-    if t.dtype != cache.dtype or t.device != cache.device:
+def _kv4_rows(cache: PagedKV4, name: str, t: torch.Tensor, T: int, heads: int) -> tuple[int, int, int]:
+    """(address, token stride, head stride) of a [T, heads, D] operand after its checks."""
+    if t.shape != (T, heads, cache.head_dim):
+        raise RuntimeError(f"{name} must be [{T}, {heads}, {cache.head_dim}]")
+    if t.dtype is not cache.dtype or t.get_device() != cache.index:
         raise RuntimeError(f"{name} must be a {cache.dtype} tensor on {cache.device}")
     st, sh, sd = t.stride()
-    if (sd != 1 or st % 8 or sh % 8 or t.data_ptr() % 16) and t.numel():
+    at = t.data_ptr()
+    if (sd != 1 or st % 8 or sh % 8 or at % 16) and t.numel():
         raise RuntimeError(f"{name} needs unit stride in its last dimension, other strides a multiple of 8 and "
                            "16-byte alignment")
+    return at, st, sh
 
 
 def kv4_append(cache: PagedKV4, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
@@ -463,20 +465,20 @@ def kv4_append(cache: PagedKV4, q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
     position or page out of range is left out and raises bit 2 of `device_status`."""
     if q.dim() != 3:
         raise RuntimeError("q must be [T, heads, D]")
-    T, dev = q.shape[0], cache.device
-    for name, t, heads in (("q", q, None), ("k", k, cache.kv_heads), ("v", v, cache.kv_heads)):
-        _kv4_rows(cache, name, t, T, heads)
+    T, heads, D = q.shape
+    at = (*_kv4_rows(cache, "q", q, T, heads), *_kv4_rows(cache, "k", k, T, cache.kv_heads),
+          *_kv4_rows(cache, "v", v, T, cache.kv_heads))
     _no_grad_inputs(q, k, v)
-    for name, t in (("cos", cos), ("sin", sin)):
-        if t.dim() != 2 or t.shape != cos.shape or t.shape[1] != cache.head_dim or not t.is_contiguous():
-            raise RuntimeError(f"{name} must be a contiguous [positions, {cache.head_dim}] table")
-        if t.dtype not in (cache.dtype, torch.float32) or t.dtype != cos.dtype or t.device != dev:
-            raise RuntimeError(f"cos and sin must both be {cache.dtype} or both float32, on {dev}")
+    table, tab = cos.shape, cos.dtype
+    if len(table) != 2 or table[1] != D or sin.shape != table or not (cos.is_contiguous() and sin.is_contiguous()):
+        raise RuntimeError(f"cos and sin must be contiguous [positions, {cache.head_dim}] tables")
+    if (tab is not cache.dtype and tab is not torch.float32) or sin.dtype is not tab or \
+            cos.get_device() != cache.index or sin.get_device() != cache.index:
+        raise RuntimeError(f"cos and sin must both be {cache.dtype} or both float32, on {cache.device}")
     batch = _kv4_batch(cache, page_table, q_start, lengths)
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    rc = _launch(dev, _lib.load().dscq_kv4_append, batch, q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2],
-                 v.data_ptr(), *v.stride()[:2], T, q.shape[1], cos.data_ptr(), sin.data_ptr(), _DT[cos.dtype],
-                 cos.shape[0], out.data_ptr())
+    out = torch.empty((T, heads, D), dtype=cache.dtype, device=cache.device)
+    rc = _launch(cache.device, _lib.load().dscq_kv4_append, batch, *at, T, heads, cos.data_ptr(), sin.data_ptr(),
+                 _DT[tab], table[0], out.data_ptr())
     _lib.check(rc, "kv4_append")
     return out
 
@@ -499,11 +501,9 @@ _kv4_space: dict = {}
 
 
 def _kv4_workspace(dev: torch.device, head_dim: int) -> int:
-    key = (dev.index, head_dim)
-    if key not in _kv4_space:
-        with torch.cuda.device(dev):
-            _kv4_space[key] = _lib.load().dscq_kv4_attention_workspace(head_dim)
-    return _kv4_space[key]
+    with torch.cuda.device(dev):
+        size = _kv4_space[(dev.index, head_dim)] = _lib.load().dscq_kv4_attention_workspace(head_dim)
+    return size
 
 
 def kv4_attention(cache: PagedKV4, q: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor,
@@ -516,19 +516,20 @@ def kv4_attention(cache: PagedKV4, q: torch.Tensor, page_table: torch.Tensor, q_
     sequence has in this call (default T). Rows of no sequence, and rows that see no key, are zero."""
     if q.dim() != 3:
         raise RuntimeError("q must be [T, heads, D]")
-    T, dev = q.shape[0], cache.device
-    _kv4_rows(cache, "q", q, T, None)
+    T, heads, D = q.shape
+    at = _kv4_rows(cache, "q", q, T, heads)
     _no_grad_inputs(q)
-    if q.shape[1] % cache.kv_heads or q.shape[1] == 0:
+    if heads % cache.kv_heads or heads == 0:
         raise RuntimeError("q's heads must be a multiple of the cache's")
     if max_q is not None and max_q < 0:
         raise RuntimeError("max_q must not be negative")
     batch = _kv4_batch(cache, page_table, q_start, lengths)
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    size = _kv4_workspace(dev, cache.head_dim)
+    dev = cache.device
+    out = torch.empty((T, heads, D), dtype=cache.dtype, device=dev)
+    size = _kv4_space.get((cache.index, D)) or _kv4_workspace(dev, D)
     space = torch.empty(size, dtype=torch.uint8, device=dev)  # this call's own: calls may overlap, graphs keep theirs
-    rc = _launch(dev, _lib.load().dscq_kv4_attention, batch, q.data_ptr(), *q.stride()[:2], T, q.shape[1], max_q or 0,
-                 cache.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(), space.data_ptr(), size)
+    rc = _launch(dev, _lib.load().dscq_kv4_attention, batch, *at, T, heads, max_q or 0,
+                 D ** -0.5 if scale is None else float(scale), out.data_ptr(), space.data_ptr(), size)
     _lib.check(rc, "kv4_attention")
     return out
 
@@ -551,21 +552,21 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) 
     if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in _DT:
         raise RuntimeError("logits must be a 2-D bf16, f16 or f32 CUDA tensor")
     rows, V = logits.shape
-    if logits.numel() and ((V > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < V)):
+    ld, step = logits.stride()
+    if ((V > 1 and step != 1) or (rows > 1 and ld < V)) and logits.numel():
         raise RuntimeError("logits need unit column stride and rows that do not overlap")
-    if targets.dtype != torch.int64 or targets.shape != (rows,) or targets.device != logits.device or \
+    dev = logits.device
+    if targets.dtype is not torch.int64 or targets.shape != (rows,) or targets.get_device() != dev.index or \
             not targets.is_contiguous():
-        raise RuntimeError(f"targets must be a contiguous int64 tensor [{rows}] on {logits.device}")
-    if not 0 <= top_k <= min(64, V):
+        raise RuntimeError(f"targets must be a contiguous int64 tensor [{rows}] on {dev}")
+    if not 0 <= top_k <= 64 or top_k > V:
         raise RuntimeError("need 0 <= top_k <= 64 and top_k <= V")
     _no_grad_inputs(logits)
-    dev = logits.device
     stats = torch.empty((2, rows), dtype=torch.float32, device=dev)
     top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
     ids = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
     at = stats.data_ptr()
     rc = _launch(dev, _lib.load().dscq_token_logprobs, logits.data_ptr(), _DT[logits.dtype], rows, V,
-                 logits.stride(0) if rows > 1 else V, targets.data_ptr(), top_k, at, at + 4 * rows, top.data_ptr(),
-                 ids.data_ptr())
+                 ld if rows > 1 else V, targets.data_ptr(), top_k, at, at + 4 * rows, top.data_ptr(), ids.data_ptr())
     _lib.check(rc, "token_logprobs")
     return TokenLogprobs(*stats.unbind(0), top, ids)

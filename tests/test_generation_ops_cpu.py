@@ -11,7 +11,7 @@ def batch(p, **changes):
     fields = dict(k_codes=p, k_affine=p, v_codes=p, v_affine=p, pages=4, kv_heads=2, page_size=64, head_dim=128,
                   dtype=_lib.BF16, page_table=p, ld_table=3, max_pages=3, q_start=p, lengths=p, seqs=2)
     fields.update(changes)
-    return _lib.Kv4Batch(**fields)
+    return _lib.KV4_BATCH.pack(*(v or 0 for v in fields.values()))
 
 
 @pytest.fixture
