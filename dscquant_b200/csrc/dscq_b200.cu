@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -522,19 +523,34 @@ cudaError_t launch_kv4_read(const dscq::Kv4Batch& b, int64_t rows, void* k, void
 template <int D, int NT>
 using Kv4Decode = dscq::Kv4DecodeConfig<D, NT, NT == 1 ? 12 : 8, 2, 64>;
 
+// cudaFuncAttributeMaxDynamicSharedMemorySize, set once per kernel and device (`done` is the kernel's own).
+cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_acquire) >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+  return e;
+}
+
 template <typename T, int D, int NT>
 cudaError_t launch_kv4_decode(const dscq::Kv4AttnParams& a, int64_t max_rows, void* ws, cudaStream_t st) {
   using C = Kv4Decode<D, NT>;
-  const int parts = num_sms();
-  dscq::Kv4DecodeParams p{a, max_rows, static_cast<float*>(ws), nullptr, nullptr};
+  static std::atomic<uint64_t> ready{0};
+  const int sms = num_sms();
+  // A CTA per run and no second kernel, where the grid can hold every run and no run can be longer than two tiles
+  // a warp.
+  const int64_t runs = (static_cast<int64_t>(a.T) * a.group / C::RB + std::min(a.b.B, a.T)) * a.b.hk;
+  const bool whole = runs <= sms && (static_cast<int64_t>(a.b.P) << a.b.ps_log2) <= 2 * C::WARPS * C::TILE;
+  const int parts = sms;
+  dscq::Kv4DecodeParams p{a, max_rows, static_cast<float*>(ws), nullptr, nullptr, whole};
   p.warp = p.cta + static_cast<int64_t>(parts) * 2 * C::kPiece;
   p.desc = reinterpret_cast<int*>(p.warp + static_cast<int64_t>(parts) * C::WARPS * C::kPiece);
-  cudaError_t e = cudaFuncSetAttribute(dscq::kv4_decode_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       C::kSmem);
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(dscq::kv4_decode_kernel<T, C>), C::kSmem, ready);
   if (e != cudaSuccess) return e;
   dscq::kv4_decode_kernel<T, C><<<parts, C::WARPS * 32, C::kSmem, st>>>(p);
   e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || whole) return e;
   // launched while the first kernel still runs; waits for its results on the device
   cudaLaunchAttribute early{};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -563,7 +579,8 @@ cudaError_t launch_kv4_attention(const dscq::Kv4AttnParams& a, int64_t max_q, vo
   if (e != cudaSuccess) return e;
   const dscq::Kv4PromptParams p{a, few + 1};
   constexpr int smem = dscq::Kv4PromptConfig<D>::kSmem;
-  e = cudaFuncSetAttribute(dscq::kv4_prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> ready{0};
+  e = allow_smem(reinterpret_cast<const void*>(dscq::kv4_prompt_kernel<T, D>), smem, ready);
   if (e != cudaSuccess) return e;
   dscq::kv4_prompt_kernel<T, D><<<static_cast<unsigned>(ctas), dscq::kKv4PromptThreads, smem, st>>>(p);
   return cudaGetLastError();

@@ -32,6 +32,7 @@ struct Kv4DecodeParams {
   float* cta;        // [G][2] pieces of runs cut by CTA borders
   float* warp;       // [G][WARPS] pieces of runs cut at a warp's start
   int* desc;         // [G][8]: slot 0 {valid, ends}, slot 1 {valid, b, h, block}
+  int whole;         // a CTA takes a whole run (the grid holds all of them): no run is cut by a CTA border
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -172,7 +173,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
   uint32_t* vmask_all = reinterpret_cast<uint32_t*>(bars + WARPS * STAGES);
   __shared__ int64_t scan[WARPS];
   __shared__ int64_t tiles_before[WARPS * 32];  // of each thread's sequences
-  __shared__ int piece[2 * WARPS][6];  // valid, starts, ends, b, h, block; pieces 2w (cut at its start), 2w + 1
+  __shared__ int piece[2 * WARPS][6];  // where (0: none), starts, ends, b, h, block; pieces 2w (cut at its start), 2w + 1
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   uint8_t* ring = kv4_smem + warp * C::kRing;
@@ -196,30 +197,42 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
     }
   }
 
-  // Every CTA adds up the tiles of all sequences; whoever holds a warp's first tile says where it is.
-  const int per = (B + WARPS * 32 - 1) / (WARPS * 32);
-  const int s_lo = min(tid * per, B), s_hi = min(s_lo + per, B);
+  // Adds up what all sequences hold (tiles, or runs where a CTA takes a whole one) and finds the warp's share: the
+  // sequences [s_lo, s_hi) its first tile is in, `left` tiles (runs) from the start of the first. Up to 256 sequences
+  // every warp does it alone, more are added up by the whole CTA.
+  auto units_of = [&](const Kv4Seq& r) {
+    return static_cast<int64_t>(r.blocks) * a.b.hk * (p.whole ? 1 : r.tiles);
+  };
+  auto scan32 = [&](int64_t v) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    return v;
+  };
+  const bool alone = B <= 256;
+  const int adders = alone ? 32 : WARPS * 32, adder = alone ? lane : tid;
+  const int per = (B + adders - 1) / adders;
   int64_t mine = 0;
-  for (int s = s_lo; s < s_hi; ++s) {
-    const Kv4Seq r = kv4_seq<TILE, RB>(a, p.max_rows, s);
-    mine += static_cast<int64_t>(r.blocks) * r.tiles * a.b.hk;
-  }
-  int64_t incl = mine;
+  for (int s = min(adder * per, B); s < min(adder * per + per, B); ++s)
+    mine += units_of(kv4_seq<TILE, RB>(a, p.max_rows, s));
+  const int64_t incl = scan32(mine);
+  int64_t total, before = incl - mine;
+  if (alone) {
+    total = __shfl_sync(0xffffffffu, incl, 31);
+  } else {
+    if (lane == 31) scan[warp] = incl;
+    __syncthreads();
+    total = 0;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
+    for (int w = 0; w < WARPS; ++w) {
+      if (w == warp) before += total;
+      total += scan[w];
+    }
+    tiles_before[tid] = before;
+    __syncthreads();
   }
-  if (lane == 31) scan[warp] = incl;
-  __syncthreads();
-  int64_t total = 0, before = 0;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    if (w == warp) before = total;
-    total += scan[w];
-  }
-  before += incl - mine;
-  tiles_before[tid] = before;
   // Equal shares: warp g of the launch begins at tile g * base + min(g, extra). A warp has at least one tile
   // where there are enough; CTAs beyond that have none.
   const int parts = static_cast<int>(max(min(total / WARPS, static_cast<int64_t>(gridDim.x)), static_cast<int64_t>(1)));
@@ -227,34 +240,32 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
   const int64_t base = total >> 32 ? total / shares : static_cast<uint32_t>(total) / static_cast<uint32_t>(shares);
   const int extra = static_cast<int>(total - base * shares);
   const int gw = blockIdx.x * WARPS + warp;
-  const int count = gw < shares ? static_cast<int>(base) + (gw < extra) : 0;
-  __syncthreads();
+  int count = gw < shares ? static_cast<int>(base) + (gw < extra) : 0;
   struct Cursor {
     int b, h, blk, t;
     Kv4Seq s;
   };
   Cursor c{};
-  if (count > 0) {
-    // The thread whose sequences hold the warp's first tile, then the sequence among them.
-    int64_t left = gw * base + min(gw, extra);
-    unsigned le = __ballot_sync(0xffffffffu, tiles_before[lane * WARPS] <= left);
-    int th = (31 - __clz(le)) * WARPS;
-    le = __ballot_sync(0xffffffffu, lane < WARPS && tiles_before[th + (lane < WARPS ? lane : 0)] <= left);
-    th += 31 - __clz(le);
-    left -= tiles_before[th];
+  if (p.whole ? static_cast<int64_t>(blockIdx.x) < total : count > 0) {
+    int64_t left = p.whole ? static_cast<int64_t>(blockIdx.x) : gw * base + min(gw, extra);
+    int th;
+    if (alone) {
+      th = 31 - __clz(__ballot_sync(0xffffffffu, before <= left));
+      left -= __shfl_sync(0xffffffffu, before, th);
+    } else {
+      unsigned le = __ballot_sync(0xffffffffu, tiles_before[lane * WARPS] <= left);
+      th = (31 - __clz(le)) * WARPS;
+      le = __ballot_sync(0xffffffffu, lane < WARPS && tiles_before[th + (lane < WARPS ? lane : 0)] <= left);
+      th += 31 - __clz(le);
+      left -= tiles_before[th];
+    }
+    const int s_hi = min(th * per + per, B);
     for (int s0 = th * per;; s0 += 32) {
-      const int s = s0 + lane;
       Kv4Seq r{};
-      if (s < min(th * per + per, B)) r = kv4_seq<TILE, RB>(a, p.max_rows, s);
-      const int64_t units = static_cast<int64_t>(r.blocks) * r.tiles * a.b.hk;
-      int64_t upto = units;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
-      }
+      if (s0 + lane < s_hi) r = kv4_seq<TILE, RB>(a, p.max_rows, s0 + lane);
+      const int64_t units = units_of(r), upto = scan32(units);
       const unsigned past = __ballot_sync(0xffffffffu, upto > left);
-      if (!past && s0 + 32 < min(th * per + per, B)) {
+      if (!past && s0 + 32 < s_hi) {
         left -= __shfl_sync(0xffffffffu, upto, 31);
         continue;
       }
@@ -269,11 +280,23 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
       c.s.keys = __shfl_sync(0xffffffffu, r.keys, src);
       break;
     }
-    const int64_t run = left >> 32 ? left / c.s.tiles : static_cast<uint32_t>(left) / static_cast<uint32_t>(c.s.tiles);
-    c.t = static_cast<int>(left - run * c.s.tiles);
+    int64_t run = left;
+    if (p.whole) {
+      const int n = c.s.tiles / WARPS, more = c.s.tiles % WARPS;
+      count = n + (warp < more);
+      c.t = warp * n + min(warp, more);
+    } else {
+      run = left >> 32 ? left / c.s.tiles : static_cast<uint32_t>(left) / static_cast<uint32_t>(c.s.tiles);
+      c.t = static_cast<int>(left - run * c.s.tiles);
+    }
     c.h = static_cast<int>(run >> 32 ? run / c.s.blocks : static_cast<uint32_t>(run) / static_cast<uint32_t>(c.s.blocks));
     c.blk = static_cast<int>(run - static_cast<int64_t>(c.h) * c.s.blocks);
+  } else {
+    count = 0;
   }
+  // sequences that share rows can have more runs than the grid was made for
+  if (p.whole && total > gridDim.x && tid == 0) raise_status(kStatusBadIndex);
+  if (alone) __syncthreads();  // the barriers and pieces set up above
   Cursor pr = c;  // the tile to fetch next
   auto advance = [&](Cursor& x, bool more) {  // more: there is a tile behind this one
     if (++x.t < x.s.tiles) return;
@@ -588,7 +611,8 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
       // ---- a run (or a piece of one) is done
       const bool whole = t0 == 0 && run_ends;
       const int slot = t0 > 0 ? 0 : 1;
-      float* dst = slot == 0 ? first_all + warp * C::kPiece : reinterpret_cast<float*>(ring);
+      const bool last = i + 1 == count;  // the ring is free then, an earlier piece goes through the cache
+      float* dst = last ? reinterpret_cast<float*>(ring) : first_all + warp * C::kPiece;
       const float back = pow2f(vexp);  // 2^-24 of the codes and 2^(14 - vexp) of the weights, undone in two steps
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -632,7 +656,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
         pc[1] = t0 == 0;
         pc[2] = run_ends;
         pc[3] = c.b, pc[4] = c.h, pc[5] = c.blk;
-        pc[0] = 1;
+        pc[0] = last ? 2 : 1;
       }
     }
     advance(c, i + 1 < count);
@@ -675,8 +699,8 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
     y.clear();
     for (unsigned x = group; x; x &= x - 1) {
       const int i = __ffs(x) - 1;
-      y.add(i & 1 ? reinterpret_cast<const float*>(kv4_smem + (i >> 1) * C::kRing) : first_all + (i >> 1) * C::kPiece,
-            RB, row0, lane);
+      y.add(piece[i][0] == 2 ? reinterpret_cast<const float*>(kv4_smem + (i >> 1) * C::kRing)
+                             : first_all + (i >> 1) * C::kPiece, RB, row0, lane);
     }
     const int* hd = piece[head];
     const bool starts = hd[1], ends = piece[31 - __clz(group)][2];

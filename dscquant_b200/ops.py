@@ -476,7 +476,7 @@ def kv4_append(cache: PagedKV4, q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
             cos.get_device() != cache.index or sin.get_device() != cache.index:
         raise RuntimeError(f"cos and sin must both be {cache.dtype} or both float32, on {cache.device}")
     batch = _kv4_batch(cache, page_table, q_start, lengths)
-    out = torch.empty((T, heads, D), dtype=cache.dtype, device=cache.device)
+    out = q.new_empty((T, heads, D))
     rc = _launch(cache.device, _lib.load().dscq_kv4_append, batch, *at, T, heads, cos.data_ptr(), sin.data_ptr(),
                  _DT[tab], table[0], out.data_ptr())
     _lib.check(rc, "kv4_append")
@@ -525,7 +525,7 @@ def kv4_attention(cache: PagedKV4, q: torch.Tensor, page_table: torch.Tensor, q_
         raise RuntimeError("max_q must not be negative")
     batch = _kv4_batch(cache, page_table, q_start, lengths)
     dev = cache.device
-    out = torch.empty((T, heads, D), dtype=cache.dtype, device=dev)
+    out = q.new_empty((T, heads, D))
     size = _kv4_space.get((cache.index, D)) or _kv4_workspace(dev, D)
     space = torch.empty(size, dtype=torch.uint8, device=dev)  # this call's own: calls may overlap, graphs keep theirs
     rc = _launch(dev, _lib.load().dscq_kv4_attention, batch, *at, T, heads, max_q or 0,
@@ -562,9 +562,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0) 
     if not 0 <= top_k <= 64 or top_k > V:
         raise RuntimeError("need 0 <= top_k <= 64 and top_k <= V")
     _no_grad_inputs(logits)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=dev)
-    top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
-    ids = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
+    stats = targets.new_empty((2, rows), dtype=torch.float32)
+    top = targets.new_empty((rows, top_k), dtype=torch.float32)
+    ids = targets.new_empty((rows, top_k))
     at = stats.data_ptr()
     rc = _launch(dev, _lib.load().dscq_token_logprobs, logits.data_ptr(), _DT[logits.dtype], rows, V,
                  ld if rows > 1 else V, targets.data_ptr(), top_k, at, at + 4 * rows, top.data_ptr(), ids.data_ptr())
