@@ -22,6 +22,7 @@
 // CTA are done, pieces of runs cut by CTA borders in a second kernel, in order: no atomics, the same bits every time.
 #pragma once
 #include "kv4_attention.cuh"
+#include "rotq_tc.cuh"
 
 namespace dscq {
 
@@ -86,39 +87,58 @@ template <int D>
 struct Kv4Joined {
   static constexpr int E = D / 32;
   float m[4], l[4], y[4][E];
-  __device__ __forceinline__ void clear() {
+  // Pieces `which` (bits), at(i) giving piece i: lane i weighs piece i, then all add them up.
+  template <class At>
+  __device__ __forceinline__ void join(unsigned which, At at, int RB, int row0, int lane) {
+    float pm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, pl[4] = {0.f, 0.f, 0.f, 0.f}, f[4];
+    if (which >> lane & 1u) {
+      const float* piece = at(lane);
+      const float4 a = *reinterpret_cast<const float4*>(piece + RB * D + row0);
+      const float4 b = *reinterpret_cast<const float4*>(piece + RB * D + RB + row0);
+      pm[0] = a.x, pm[1] = a.y, pm[2] = a.z, pm[3] = a.w;
+      pl[0] = b.x, pl[1] = b.y, pl[2] = b.z, pl[3] = b.w;
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      m[r] = -INFINITY;
-      l[r] = 0.f;
+      m[r] = pm[r];
+#pragma unroll
+      for (int o = 16; o; o >>= 1) m[r] = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], o));
+      f[r] = ex2(pm[r] - (m[r] == -INFINITY ? 0.f : m[r]));
+      l[r] = pl[r] * f[r];
+#pragma unroll
+      for (int o = 16; o; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
 #pragma unroll
       for (int e = 0; e < E; ++e) y[r][e] = 0.f;
     }
-  }
-  __device__ __forceinline__ void add(const float* piece, int RB, int row0, int lane) {
-    const float4 pm = *reinterpret_cast<const float4*>(piece + RB * D + row0);
-    const float4 pl = *reinterpret_cast<const float4*>(piece + RB * D + RB + row0);
-    const float ms[4] = {pm.x, pm.y, pm.z, pm.w}, ls[4] = {pl.x, pl.y, pl.z, pl.w};
-    float x[4][E];
+    for (unsigned x = which; x; x &= x - 1) {
+      const int i = __ffs(x) - 1;
+      const float* src = at(i) + row0 * D + lane * E;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float* src = piece + (row0 + r) * D + lane * E;
-      if constexpr (E == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(src);
-        x[r][0] = v.x, x[r][1] = v.y, x[r][2] = v.z, x[r][3] = v.w;
-      } else {
-        const float2 v = *reinterpret_cast<const float2*>(src);
-        x[r][0] = v.x, x[r][1] = v.y;
+      for (int r = 0; r < 4; ++r) {
+        const float g = __shfl_sync(0xffffffffu, f[r], i);
+        float v[E];
+        if constexpr (E == 4) {
+          const float4 u = *reinterpret_cast<const float4*>(src + r * D);
+          v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+        } else {
+          const float2 u = *reinterpret_cast<const float2*>(src + r * D);
+          v[0] = u.x, v[1] = u.y;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[r][e] = fmaf(v[e], g, y[r][e]);
       }
     }
+  }
+  // The same with `other`, earlier pieces first.
+  __device__ __forceinline__ void add(const Kv4Joined& other) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const float n = fmaxf(m[r], ms[r]), nb = n == -INFINITY ? 0.f : n;
-      const float f = ex2(m[r] - nb), g = ex2(ms[r] - nb);
+      const float n = fmaxf(m[r], other.m[r]), nb = n == -INFINITY ? 0.f : n;
+      const float f = ex2(m[r] - nb), g = ex2(other.m[r] - nb);
       m[r] = n;
-      l[r] = fmaf(l[r], f, ls[r] * g);
+      l[r] = fmaf(l[r], f, other.l[r] * g);
 #pragma unroll
-      for (int e = 0; e < E; ++e) y[r][e] = fmaf(y[r][e], f, x[r][e] * g);
+      for (int e = 0; e < E; ++e) y[r][e] = fmaf(y[r][e], f, other.y[r][e] * g);
     }
   }
   __device__ __forceinline__ void store(float* piece, int RB, int row0, int lane) const {
@@ -185,18 +205,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
   }
   if (tid < 2 * WARPS) piece[tid][0] = 0;
 
-  // Rows of no sequence are zero.
   const int B = a.b.B;
-  {
-    const int lo = B ? min(max(a.b.q_start[0], 0), a.T) : 0, hi = B ? min(max(a.b.q_start[B], lo), a.T) : 0;
-    const int64_t row16 = static_cast<int64_t>(a.hq) * D / 8;  // 16-byte pieces of a row
-    const int64_t none = (lo + a.T - hi) * row16;
-    for (int64_t i = blockIdx.x * (WARPS * 32ll) + tid; i < none; i += gridDim.x * (WARPS * 32ll)) {
-      const int64_t r = i < lo * row16 ? i : i - lo * row16 + hi * row16;
-      reinterpret_cast<uint4*>(a.out)[r] = make_uint4(0, 0, 0, 0);
-    }
-  }
-
   // Adds up what all sequences hold (tiles, or runs where a CTA takes a whole one) and finds the warp's share: the
   // sequences [s_lo, s_hi) its first tile is in, `left` tiles (runs) from the start of the first. Up to 256 sequences
   // every warp does it alone, more are added up by the whole CTA.
@@ -215,8 +224,11 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
   const int adders = alone ? 32 : WARPS * 32, adder = alone ? lane : tid;
   const int per = (B + adders - 1) / adders;
   int64_t mine = 0;
-  for (int s = min(adder * per, B); s < min(adder * per + per, B); ++s)
-    mine += units_of(kv4_seq<TILE, RB>(a, p.max_rows, s));
+  Kv4Seq held{};  // the adder's (last) sequence
+  for (int s = min(adder * per, B); s < min(adder * per + per, B); ++s) {
+    held = kv4_seq<TILE, RB>(a, p.max_rows, s);
+    mine += units_of(held);
+  }
   const int64_t incl = scan32(mine);
   int64_t total, before = incl - mine;
   if (alone) {
@@ -260,7 +272,19 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
       left -= tiles_before[th];
     }
     const int s_hi = min(th * per + per, B);
-    for (int s0 = th * per;; s0 += 32) {
+    auto take = [&](const Kv4Seq& r, int src) {
+      c.s.q0 = __shfl_sync(0xffffffffu, r.q0, src);
+      c.s.n = __shfl_sync(0xffffffffu, r.n, src);
+      c.s.len = __shfl_sync(0xffffffffu, r.len, src);
+      c.s.tiles = max(__shfl_sync(0xffffffffu, r.tiles, src), 1);
+      c.s.blocks = max(__shfl_sync(0xffffffffu, r.blocks, src), 1);
+      c.s.keys = __shfl_sync(0xffffffffu, r.keys, src);
+    };
+    if (alone && per == 1) {
+      c.b = th;
+      take(held, th);
+    }
+    for (int s0 = th * per; !(alone && per == 1); s0 += 32) {
       Kv4Seq r{};
       if (s0 + lane < s_hi) r = kv4_seq<TILE, RB>(a, p.max_rows, s0 + lane);
       const int64_t units = units_of(r), upto = scan32(units);
@@ -272,12 +296,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
       const int src = past ? __ffs(past) - 1 : 31;
       left -= __shfl_sync(0xffffffffu, upto - units, src);
       c.b = s0 + src;
-      c.s.q0 = __shfl_sync(0xffffffffu, r.q0, src);
-      c.s.n = __shfl_sync(0xffffffffu, r.n, src);
-      c.s.len = __shfl_sync(0xffffffffu, r.len, src);
-      c.s.tiles = max(__shfl_sync(0xffffffffu, r.tiles, src), 1);
-      c.s.blocks = max(__shfl_sync(0xffffffffu, r.blocks, src), 1);
-      c.s.keys = __shfl_sync(0xffffffffu, r.keys, src);
+      take(r, src);
       break;
     }
     int64_t run = left;
@@ -351,6 +370,17 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
     }
   };
   while (fetched < STAGES && fetched < count) fetch_next(fetched);
+
+  // Rows of no sequence are zero.
+  {
+    const int lo = B ? min(max(a.b.q_start[0], 0), a.T) : 0, hi = B ? min(max(a.b.q_start[B], lo), a.T) : 0;
+    const int64_t row16 = static_cast<int64_t>(a.hq) * D / 8;  // 16-byte pieces of a row
+    const int64_t none = (lo + a.T - hi) * row16;
+    for (int64_t i = blockIdx.x * (WARPS * 32ll) + tid; i < none; i += gridDim.x * (WARPS * 32ll)) {
+      const int64_t r = i < lo * row16 ? i : i - lo * row16 + hi * row16;
+      reinterpret_cast<uint4*>(a.out)[r] = make_uint4(0, 0, 0, 0);
+    }
+  }
 
   // mx is the running maximum of the scores in their rows' own units, c1 turns those into powers of two
   float o[NT][D / 16][4], mx[NT][2], l[NT][2], low[NT][2], sumq[NT][2], c1[NT][2];
@@ -443,13 +473,23 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int at = 16 * kb + 8 * j + g;
-        va[kb][j] = vaff[at];
-        // what no row sees may hold anything
-        if (masked && (key0 + at >= max_lim || !((have >> (at >> pl2)) & 1u))) va[kb][j] = 0;
-        vmax = fmaxf(vmax, unpack2<T>(va[kb][j]).x);
-      }
+      for (int j = 0; j < 2; ++j) va[kb][j] = vaff[16 * kb + 8 * j + g];
+    bool poison = false;  // keys some rows see and others do not, with values that are no numbers
+    if (masked) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int at = 16 * kb + 8 * j + g;
+          // what no row sees may hold anything
+          if (key0 + at >= max_lim || !((have >> (at >> pl2)) & 1u)) va[kb][j] = 0;
+          const float2 f = unpack2<T>(va[kb][j]);
+          poison |= !isfinite(f.x) || !isfinite(f.y);
+        }
+      poison = __any_sync(0xffffffffu, poison);
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) vmax = fmax3(vmax, unpack2<T>(va[kb][0]).x, unpack2<T>(va[kb][1]).x);
     float shrink = 1.f;
     if (__any_sync(0xffffffffu, vmax >= pow2f(vexp))) {
 #pragma unroll
@@ -519,13 +559,12 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
       float al[2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        float m = fmaxf(s[nt][0][x], s[nt][0][2 + x]);
+        float m = mx[nt][x];
 #pragma unroll
-        for (int kb = 1; kb < KB; ++kb) m = fmaxf(m, fmaxf(s[nt][kb][x], s[nt][kb][2 + x]));
+        for (int kb = 0; kb < KB; ++kb) m = fmax3(m, s[nt][kb][x], s[nt][kb][2 + x]);
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-        m = fmaxf(m, mx[nt][x]);
         base[nt][x] = m == -INFINITY ? 0.f : m * c1[nt][x];
         al[x] = mx[nt][x] == m ? 1.f : ex2(fmaf(mx[nt][x], c1[nt][x], -base[nt][x]));
         mx[nt][x] = m;
@@ -554,18 +593,23 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float w[4];
+        float pe[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float pe = ex2(fmaf(s[nt][kb][e], c1[nt][e & 1], -base[nt][e & 1]));
-          l[nt][e & 1] += pe;
-          w[e] = pe * (e < 2 ? f0 : f1);
-          if (!masked) {
-            low[nt][e & 1] = fmaf(pe, e < 2 ? v0.y : v1.y, low[nt][e & 1]);
-          } else if (s[nt][kb][e] == -INFINITY) {
-            w[e] = 0.f;  // a key this row does not see may be NaN to others
-          } else {
-            low[nt][e & 1] = fmaf(pe, e < 2 ? v0.y : v1.y, low[nt][e & 1]);
-          }
+          pe[e] = ex2(fmaf(s[nt][kb][e], c1[nt][e & 1], -base[nt][e & 1]));
+          l[nt][e & 1] += pe[e];
+          w[e] = pe[e] * (e < 2 ? f0 : f1);
+        }
+        if (!poison) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) low[nt][e & 1] = fmaf(pe[e], e < 2 ? v0.y : v1.y, low[nt][e & 1]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (s[nt][kb][e] == -INFINITY)
+              w[e] = 0.f;
+            else
+              low[nt][e & 1] = fmaf(pe[e], e < 2 ? v0.y : v1.y, low[nt][e & 1]);
         }
         bf[nt][0] = movmatrix_trans(pack2<__half>(w[0], w[1]));
         bf[nt][1] = movmatrix_trans(pack2<__half>(w[2], w[3]));
@@ -696,12 +740,10 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
     const unsigned later = rest & (rest - 1);
     const unsigned group = all & ~((1u << head) - 1) & (later ? (later & -later) - 1 : ~0u);
     Kv4Joined<D> y;
-    y.clear();
-    for (unsigned x = group; x; x &= x - 1) {
-      const int i = __ffs(x) - 1;
-      y.add(piece[i][0] == 2 ? reinterpret_cast<const float*>(kv4_smem + (i >> 1) * C::kRing)
-                             : first_all + (i >> 1) * C::kPiece, RB, row0, lane);
-    }
+    y.join(group, [&](int i) {
+      return piece[i][0] == 2 ? reinterpret_cast<const float*>(kv4_smem + (i >> 1) * C::kRing)
+                              : first_all + (i >> 1) * C::kPiece;
+    }, RB, row0, lane);
     const int* hd = piece[head];
     const bool starts = hd[1], ends = piece[31 - __clz(group)][2];
     if (starts && ends) {
@@ -732,12 +774,29 @@ __global__ void __launch_bounds__(32 * RB / 4) kv4_decode_join(const Kv4DecodePa
   const int* d0 = p.desc + blockIdx.x * 8;
   if (!d0[2]) return;
   const int row0 = (threadIdx.x >> 5) * 4, lane = threadIdx.x & 31;
+  // its pieces: the one it starts with, then the first ones of the CTAs behind, up to the one that ends it; 32 at a time
   Kv4Joined<D> y;
-  y.clear();
-  y.add(p.cta + (blockIdx.x * 2 + 1) * kPiece, RB, row0, lane);
-  for (int i = blockIdx.x + 1; i < parts && p.desc[i * 8]; ++i) {
-    y.add(p.cta + i * 2 * kPiece, RB, row0, lane);
-    if (p.desc[i * 8 + 1]) break;
+  bool more = true;
+  for (int at = blockIdx.x; more; at += 32) {
+    const int i = at + lane;
+    const bool valid = i < parts && (i == static_cast<int>(blockIdx.x) || p.desc[i * 8]);
+    const bool ends = valid && i != static_cast<int>(blockIdx.x) && p.desc[i * 8 + 1];
+    const unsigned stop = __ballot_sync(0xffffffffu, ends || !valid);
+    unsigned which = ~0u;
+    if (stop) {
+      const int k = __ffs(stop) - 1;
+      which = (1u << k) - 1;
+      if (__shfl_sync(0xffffffffu, static_cast<int>(ends), k)) which |= 1u << k;
+      more = false;
+    }
+    Kv4Joined<D> z;
+    z.join(which, [&](int j) {
+      return p.cta + ((at + j) * 2 + (at + j == static_cast<int>(blockIdx.x) ? 1 : 0)) * kPiece;
+    }, RB, row0, lane);
+    if (at == static_cast<int>(blockIdx.x))
+      y = z;
+    else
+      y.add(z);
   }
   y.template write<T>(p.a, kv4_seq<TILE, RB>(p.a, p.max_rows, d0[3]), d0[4], d0[5] * RB + row0, lane);
 }
