@@ -31,6 +31,7 @@ import torch
 import torch.nn.functional as F
 
 from . import ops
+from .kvcache import PagedKV4
 from .linear import QuantConfig, QuantLinear
 
 
@@ -95,18 +96,17 @@ class DecoderLayer:
         self.norm1 = (1.0 + 0.1 * torch.randn(H, generator=gen, device=device)).to(torch.bfloat16)
         self.norm2 = (1.0 + 0.1 * torch.randn(H, generator=gen, device=device)).to(torch.bfloat16)
 
-    def __call__(self, h: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
-        cfg = self.cfg
-        S = h.shape[0]
-        x = ops.rmsnorm(h, self.norm1, cfg.eps)
-        qx = self.q.quantize_input(x)
-        q = self.q.forward_quantized(qx, S).view(S, cfg.heads, cfg.head_dim)
-        k = self.k.forward_quantized(qx, S).view(S, cfg.kv_heads, cfg.head_dim)
-        v = self.v.forward_quantized(qx, S).view(S, cfg.kv_heads, cfg.head_dim)
-        ops.rope_(q, k, cos, sin)
-        a = F.scaled_dot_product_attention(q.transpose(0, 1)[None], k.transpose(0, 1)[None], v.transpose(0, 1)[None],
-                                           is_causal=True, enable_gqa=cfg.kv_heads != cfg.heads)
-        a = a[0].transpose(0, 1).reshape(S, cfg.hidden)
+    def project(self, h: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """q [S, heads, D], k and v [S, kv_heads, D] of the normalised input, before the rotation."""
+        cfg, S = self.cfg, h.shape[0]
+        qx = self.q.quantize_input(ops.rmsnorm(h, self.norm1, cfg.eps))
+        return (self.q.forward_quantized(qx, S).view(S, cfg.heads, cfg.head_dim),
+                self.k.forward_quantized(qx, S).view(S, cfg.kv_heads, cfg.head_dim),
+                self.v.forward_quantized(qx, S).view(S, cfg.kv_heads, cfg.head_dim))
+
+    def finish(self, h: torch.Tensor, a: torch.Tensor) -> torch.Tensor:
+        """The rest of the layer behind its attention output a [S, hidden]."""
+        cfg, S = self.cfg, h.shape[0]
         h = self.o.forward_quantized(self.o.quantize_input(a), S, residual=h)
         x = ops.rmsnorm(h, self.norm2, cfg.eps)
         gx = self.gate.quantize_input(x)
@@ -114,6 +114,23 @@ class DecoderLayer:
         u = self.up.forward_quantized(gx, S)
         m = ops.silu_mul(g, u)
         return self.down.forward_quantized(self.down.quantize_input(m), S, residual=h)
+
+    def __call__(self, h: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+        cfg, S = self.cfg, h.shape[0]
+        q, k, v = self.project(h)
+        ops.rope_(q, k, cos, sin)
+        a = F.scaled_dot_product_attention(q.transpose(0, 1)[None], k.transpose(0, 1)[None], v.transpose(0, 1)[None],
+                                           is_causal=True, enable_gqa=cfg.kv_heads != cfg.heads)
+        return self.finish(h, a[0].transpose(0, 1).reshape(S, cfg.hidden))
+
+    def step(self, h: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, cache: PagedKV4, where: tuple,
+             max_q: int | None = None) -> torch.Tensor:
+        """The layer on new tokens of a batch of sequences, keys and values kept in `cache`; `where` is
+        (page_table, q_start, lengths) as ops.kv4_append takes them, cos / sin are tables by position."""
+        q, k, v = self.project(h)
+        q = ops.kv4_append(cache, q, k, v, cos, sin, *where)
+        a = ops.kv4_attention(cache, q, *where, max_q=max_q)
+        return self.finish(h, a.view(h.shape[0], self.cfg.hidden))
 
 
 class LlamaW4A4:
@@ -149,6 +166,54 @@ class LlamaW4A4:
         """The prefill of S tokens captured once as a CUDA graph (see PrefillGraph)."""
         return PrefillGraph(self, S)
 
+    # ------------------------------------------------------------------ generation and scoring
+    def caches(self, pages: int, page_size: int = 64) -> list[PagedKV4]:
+        """An empty 4-bit cache of `pages` pages for every layer."""
+        c = self.cfg
+        return [PagedKV4.allocate(pages, c.kv_heads, c.head_dim, page_size, torch.bfloat16, self.device)
+                for _ in self.layers]
+
+    @torch.no_grad()
+    def step(self, ids: torch.Tensor, caches: list[PagedKV4], page_table: torch.Tensor, q_start: torch.Tensor,
+             lengths: torch.Tensor, max_q: int | None = None) -> torch.Tensor:
+        """Logits [T, vocab] of new tokens ids [T] of a batch of sequences (described as for ops.kv4_append;
+        `lengths` counts them in), which join the caches."""
+        cos, sin = self.rope(page_table.shape[1] * caches[0].page_size)
+        h = self.embed[ids]
+        for layer, cache in zip(self.layers, caches):
+            h = layer.step(h, cos, sin, cache, (page_table, q_start, lengths), max_q)
+        x = ops.rmsnorm(h, self.norm, self.cfg.eps)
+        return self.lm_head.forward_quantized(self.lm_head.quantize_input(x), ids.shape[0])
+
+    def generate(self, prompts: list[torch.Tensor], new_tokens: int, page_size: int = 64):
+        """Greedy continuation of each prompt (1-D ids, at least one): (ids [prompts, new_tokens], their log
+        probabilities). The prompts run as one ragged step, the tokens behind the first through DecodeGraph."""
+        counts = [len(p) for p in prompts]
+        used = [-(-(n + new_tokens) // page_size) for n in counts]
+        caches = self.caches(sum(used), page_size)
+        table = torch.full((len(prompts), max(used)), -1, dtype=torch.int32)
+        for b, n in enumerate(used):
+            table[b, :n] = torch.arange(sum(used[:b]), sum(used[:b]) + n, dtype=torch.int32)
+        table = table.to(self.device)
+        lengths = torch.tensor(counts, dtype=torch.int32, device=self.device)
+        ends = lengths.cumsum(0)
+        q_start = F.pad(ends, (1, 0)).to(torch.int32)
+        logits = self.step(torch.cat([p.to(self.device) for p in prompts]), caches, table, q_start, lengths, max(counts))
+        first = ops.token_logprobs(logits[ends - 1], torch.full_like(ends, -1), top_k=1)
+        ids, logprobs = [first.top_ids], [first.top_logprobs]
+        if new_tokens > 1:
+            graph = DecodeGraph(self, caches, table, lengths, first.top_ids[:, 0])
+            for _ in range(new_tokens - 1):
+                i, lp = graph()
+                ids.append(i.clone())
+                logprobs.append(lp.clone())
+        return torch.cat(ids[:new_tokens], 1), torch.cat(logprobs[:new_tokens], 1)
+
+    def score(self, ids: torch.Tensor, top_k: int = 0) -> "ops.TokenLogprobs":
+        """Log probability of every token of ids [S] but the first given those before it, with the entropy and the
+        top_k alternatives at each place; exp(-mean) of the log probabilities is the text's perplexity."""
+        return ops.token_logprobs(self(ids)[:-1], ids[1:].contiguous(), top_k)
+
     def linear_ops(self, S: int) -> float:
         """Integer ops of all W4A4 GEMMs of one prefill of S tokens (2 * S * N * K each)."""
         c = self.cfg
@@ -181,3 +246,40 @@ class PrefillGraph:
         self.ids.copy_(ids)
         self.graph.replay()
         return self.logits
+
+
+class DecodeGraph:
+    """One CUDA graph of a greedy decode step for a batch of sequences: each call appends the current token of every
+    sequence, runs the model over the caches and picks the next tokens, whose ids [B, 1] and log probabilities
+    come back in static buffers that the next call overwrites. Lengths and tokens advance on the device, so
+    calls need no host work; page_table must already map the positions they reach, and may be changed in place."""
+
+    def __init__(self, model: LlamaW4A4, caches: list[PagedKV4], page_table: torch.Tensor, lengths: torch.Tensor,
+                 ids: torch.Tensor):
+        dev, B = model.device, lengths.shape[0]
+        self.lengths, self.ids, self.page_table = lengths.clone(), ids.clone(), page_table
+        q_start = torch.arange(B + 1, dtype=torch.int32, device=dev)
+        nobody = torch.full((B,), -1, dtype=torch.long, device=dev)
+        self._held = model, caches, q_start, nobody  # the captured kernels go on using them
+
+        def step():
+            self.lengths.add_(1)
+            r = ops.token_logprobs(model.step(self.ids, caches, page_table, q_start, self.lengths, max_q=1), nobody, top_k=1)
+            self.ids.copy_(r.top_ids[:, 0])
+            return r.top_ids, r.top_logprobs
+
+        side = torch.cuda.Stream(dev)  # once eagerly: it builds what cannot be built in a capture, and is undone
+        side.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(side), torch.no_grad():
+            step()
+            self.lengths.copy_(lengths)
+            self.ids.copy_(ids)
+        torch.cuda.current_stream(dev).wait_stream(side)
+        torch.cuda.synchronize(dev)
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.no_grad(), torch.cuda.graph(self.graph):
+            self.out = step()
+
+    def __call__(self) -> tuple[torch.Tensor, torch.Tensor]:
+        self.graph.replay()
+        return self.out

@@ -192,6 +192,66 @@ def test_attention(cuda_device, dtype, D, heads, kv_heads, ps, mix):
     assert not out[bt.starts[-1]:].any()
 
 
+PROMPTS = {
+    "whole": [(300, 300), (129, 129), (257, 257)],
+    "chunks": [(200, 1000), (65, 3000), (1, 50), (300, 437)],
+    "empty rows": [(300, 170), (200, 0), (130, 1), (128, 128)],
+    "mixed": [(1, 700), (400, 400), (0, 9), (3, 90), (70, 71)],
+}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,heads,kv_heads,ps", [(128, 32, 32, 64), (128, 64, 8, 16), (64, 48, 16, 128), (64, 33, 11, 32)])
+@pytest.mark.parametrize("mix", PROMPTS)
+def test_attention_prompts(cuda_device, dtype, D, heads, kv_heads, ps, mix):
+    """Enough rows and heads for the tensor-core kernel, single tokens and drafts among them."""
+    from dscquant_b200 import ops
+
+    g = torch.Generator(device=cuda_device).manual_seed(11)
+    bt = Batch(PROMPTS[mix], kv_heads, D, ps, dtype, cuda_device, pad=3)
+    bt.fill(g, k_scale=1.5, v_offset=0.3)
+    q = randn((bt.T, heads, D), g, dtype, 1.5)
+    out = ops.kv4_attention(bt.cache, q, *bt.where)
+    check_attention(bt, q, out)
+    assert torch.equal(out, ops.kv4_attention(bt.cache, q, *bt.where))
+    assert not out[bt.starts[-1]:].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_prompts_with_awkward_cache(cuda_device, dtype):
+    """The tensor-core kernel on rows that are no numbers, seen or not, pages out of range, values that grow by
+    orders of magnitude along the keys, constant rows, and keys of very different sizes."""
+    from dscquant_b200 import ops
+
+    g = torch.Generator(device=cuda_device).manual_seed(12)
+    hk, D = 32, 64
+    bt = Batch([(300, 400), (260, 260)], hk, D, 16, dtype, cuda_device)
+    bt.fill(g)
+    grow = torch.logspace(-3, 3, 400, base=10 if dtype is torch.bfloat16 else 4, device=cuda_device)
+    pages, off = bt.slots(0, 0, 400)
+    bt.cache.v_affine[pages, :, off] = (bt.cache.v_affine[pages, :, off].float() * grow[:, None, None]).to(dtype)
+    flat, foff = bt.slots(1, 30, 60)
+    bt.cache.v_affine[flat, :, foff, 0] = 0  # constant rows
+    bt.cache.k_affine[flat, :, foff, 0] = 0
+    q = randn((bt.T, hk, D), g, dtype)
+    check_attention(bt, q, ops.kv4_attention(bt.cache, q, *bt.where))
+    for side in ("k_affine", "v_affine"):
+        affine = getattr(bt.cache, side)
+        kept = affine.clone()
+        pages, off = bt.slots(1, 200, 201)
+        affine[pages, :, off] = torch.nan
+        out = ops.kv4_attention(bt.cache, q, *bt.where)
+        seen = torch.zeros(bt.T, dtype=torch.bool, device=cuda_device)
+        seen[300 + 200:] = True
+        assert torch.equal(torch.isnan(out).all(-1).all(-1), seen) and torch.equal(torch.isnan(out).any(-1).any(-1), seen)
+        affine.copy_(kept)
+    want = ops.kv4_attention(bt.cache, q, *bt.where)
+    bt.table[0, 5] = bt.pages + 3
+    out = ops.kv4_attention(bt.cache, q, *bt.where)
+    assert ops.device_status(cuda_device) == 4
+    assert torch.equal(out[300:], want[300:]) and torch.isfinite(out).all()
+
+
 def test_attention_scale_strides_and_sharp_softmax(cuda_device):
     """Another scale, queries as a strided view, weights on single keys, keys far from zero."""
     from dscquant_b200 import ops
@@ -204,6 +264,11 @@ def test_attention_scale_strides_and_sharp_softmax(cuda_device):
         check_attention(bt, q, ops.kv4_attention(bt.cache, q, *bt.where, scale=0.3), 0.3)
         check_attention(bt, q, ops.kv4_attention(bt.cache, q, *bt.where, scale=0.0), 0.0)
         check_attention(bt, q, ops.kv4_attention(bt.cache, q, *bt.where, scale=-0.2), -0.2)
+        big = Batch([(150, 200), (300, 300)], 16, 128, 64, dtype, cuda_device)
+        big.fill(g, k_scale=4.0, v_offset=-3.0)
+        q = randn((big.T, 18, 128), g, dtype, 4)[:, 1:17]
+        for scale in (0.3, 0.0, -0.2):
+            check_attention(big, q, ops.kv4_attention(big.cache, q, *big.where, scale=scale), scale)
 
 
 def test_attention_shared_pages_and_wide_table(cuda_device):
