@@ -5,6 +5,8 @@
 // tensor cores multiply exactly; so an AND (and one shift for every other pair) makes two operands of two codes:
 //   q.k = step (q.n) + low sum(q)
 //   o   = sum_t P'_t n_t / F + sum_t p_t low_t,   P'_t = fp16(F p_t step_t)
+// and for f16 outputs, which would show the rounding of P' (4e-4 of the result), about the middle code, where it counts
+// a third: sum_t P'_t (n_t - 8) / F + sum_t p_t (low_t + 8 step_t), sum_t P'_t from one more product with ones.
 // No element is ever dequantised; step and low cost a few operations per key, not per element. Queries
 // enter as fp16, each row scaled by a power of two to the top of its range (exact but for elements 2^-29 below
 // the row's largest); F is a power of two that follows the largest step seen, so P' stays in range for any
@@ -58,6 +60,7 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   return y;
 }
 
+constexpr uint32_t kEight = 0x00080008u;                          // code 8 twice
 constexpr uint32_t kCode0 = 0x000F000Fu, kCode1 = 0x00F000F0u;  // two codes of a word: weights 2^-24 and 2^-20
 
 // One sequence as the decode kernel sees it.
@@ -186,6 +189,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
   constexpr int D = C::D, NT = C::NT, TILE = C::TILE, WARPS = C::WARPS, STAGES = C::STAGES, RB = C::RB;
   constexpr int KB = TILE / 16;  // 16-key blocks of a tile
   constexpr int W4 = D / 32;     // words of codes a lane takes of a key
+  constexpr bool kMid = std::is_same<T, __half>::value;  // codes about 8
   const Kv4AttnParams& a = p.a;
   extern __shared__ __align__(128) uint8_t kv4_smem[];
   float* first_all = p.warp + blockIdx.x * static_cast<int64_t>(WARPS * C::kPiece);
@@ -383,7 +387,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
   }
 
   // mx is the running maximum of the scores in their rows' own units, c1 turns those into powers of two
-  float o[NT][D / 16][4], mx[NT][2], l[NT][2], low[NT][2], sumq[NT][2], c1[NT][2];
+  float o[NT][D / 16][4], ones[NT][4], mx[NT][2], l[NT][2], low[NT][2], sumq[NT][2], c1[NT][2];
   uint32_t qf[NT][W4][4];
   int lim[NT][2], min_lim = 0, max_lim = 0, t0 = 0;
   int vexp = 0;  // every step of the values so far is below 2^vexp
@@ -444,6 +448,8 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
           mx[nt][j] = -INFINITY;
           l[nt][j] = low[nt][j] = 0.f;
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ones[nt][e] = 0.f;
 #pragma unroll
         for (int d = 0; d < D / 16; ++d)
 #pragma unroll
@@ -575,6 +581,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
           l[nt][x] *= al[x];
           low[nt][x] *= al[x];
           const float f = al[x] * shrink;
+          if constexpr (kMid) ones[nt][x] *= f;
 #pragma unroll
           for (int d = 0; d < D / 16; ++d) {
             o[nt][d][x] *= f;
@@ -589,6 +596,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
     for (int kb = 0; kb < KB; ++kb) {
       const float2 v0 = unpack2<T>(va[kb][0]), v1 = unpack2<T>(va[kb][1]);
       const float f0 = v0.x * vf, f1 = v1.x * vf;
+      const float mid0 = kMid ? fmaf(8.f, v0.x, v0.y) : v0.y, mid1 = kMid ? fmaf(8.f, v1.x, v1.y) : v1.y;
       uint32_t bf[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -602,17 +610,21 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
         }
         if (!poison) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) low[nt][e & 1] = fmaf(pe[e], e < 2 ? v0.y : v1.y, low[nt][e & 1]);
+          for (int e = 0; e < 4; ++e) low[nt][e & 1] = fmaf(pe[e], e < 2 ? mid0 : mid1, low[nt][e & 1]);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (s[nt][kb][e] == -INFINITY)
               w[e] = 0.f;
             else
-              low[nt][e & 1] = fmaf(pe[e], e < 2 ? v0.y : v1.y, low[nt][e & 1]);
+              low[nt][e & 1] = fmaf(pe[e], e < 2 ? mid0 : mid1, low[nt][e & 1]);
         }
         bf[nt][0] = movmatrix_trans(pack2<__half>(w[0], w[1]));
         bf[nt][1] = movmatrix_trans(pack2<__half>(w[2], w[3]));
+        if constexpr (kMid) {
+          const uint32_t eights[4] = {kEight, kEight, kEight, kEight};
+          mma_f16(ones[nt], eights, bf[nt][0], bf[nt][1]);
+        }
       }
       // keys 2q, 2q + 1 and 2q + 8, 2q + 9 of the block; D/8 dims from D/8 * g
       const uint8_t* vr = st + C::kCodes + (16 * kb + 2 * q) * (D / 2) + g * (D / 16);
@@ -673,8 +685,8 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
           float y[D / 8];
 #pragma unroll
           for (int d = 0; d < D / 16; ++d) {
-            y[2 * d] = fmaf(o[nt][d][x] * 0x1p10f, back, lw) * inv;
-            y[2 * d + 1] = fmaf(o[nt][d][2 + x] * 0x1p6f, back, lw) * inv;
+            y[2 * d] = fmaf((o[nt][d][x] - ones[nt][x]) * 0x1p10f, back, lw) * inv;
+            y[2 * d + 1] = fmaf((o[nt][d][2 + x] - 16.f * ones[nt][x]) * 0x1p6f, back, lw) * inv;
           }
           if (whole) {
             if (rr < rows) {

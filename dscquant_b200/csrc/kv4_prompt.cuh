@@ -11,8 +11,8 @@
 // round(n step' + low') for two elements, with (step', low') scaled by a power of two that puts the tile's largest
 // value under 2^-6 (for values: the largest so far; sums already made follow). That rounds keys and values to 11
 // bits; queries, scaled by a power of two a row, are exact. Scores, statistics and sums are 32-bit. Weights are
-// fp16, relative to a running maximum that only moves when it would be passed by 2^8: then the row's sums in
-// TMEM are scaled, by the warps that own them.
+// fp16 (11 bits, 2^-21 of the largest and more), relative to a running maximum that only moves when it would be passed by 2^8:
+// then the row's sums in TMEM are scaled, by the warps that own them.
 //
 // Keys no row may see (behind the end, on pages out of range) are zeros with their scores masked. A value row that is
 // not finite is zeros too and flagged; rows that see its key become NaN, the others must not.
@@ -257,7 +257,8 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
             }
           }
           // ---- weights, over the scores they come from
-          const float base = m == -INFINITY ? 0.f : m;
+          // weights up to 2^15: small ones stay normal fp16 numbers down to 2^-21 of the largest
+          const float base = m == -INFINITY ? 0.f : m - 7.f;
           uint32_t v[2][32];
           tmem_ld32(s_at, v[0]);
 #pragma unroll
