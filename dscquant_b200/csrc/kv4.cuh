@@ -85,22 +85,36 @@ struct Kv4Where {
   bool bad;
 };
 
-__device__ __forceinline__ Kv4Where kv4_where(const Kv4Batch& b, int t) {
+// The sequence and position of row t, for a whole warp. Up to 32 sequences take one trip to memory.
+__device__ __forceinline__ Kv4Where kv4_position(const Kv4Batch& b, int t) {
   Kv4Where w{-1, 0, 0, false};
   if (b.B == 0) return w;
-  const int s = kv4_find_seq(b.q_start, b.B, t);
-  const int q0 = b.q_start[s], q1 = b.q_start[s + 1], len = b.lengths[s];
-  if (t < q0 || t >= q1) return w;
+  int s, q1, len;
+  if (b.B <= 32) {
+    const int lane = threadIdx.x & 31, i = min(lane, b.B - 1);
+    const int lo = b.q_start[i], hi = b.q_start[i + 1], n = b.lengths[i];
+    const unsigned in = __ballot_sync(0xffffffffu, lane < b.B && t >= lo && t < hi);
+    if (!in) return w;
+    s = __ffs(in) - 1;
+    q1 = __shfl_sync(0xffffffffu, hi, s);
+    len = __shfl_sync(0xffffffffu, n, s);
+  } else {
+    s = kv4_find_seq(b.q_start, b.B, t);
+    const int q0 = b.q_start[s];
+    q1 = b.q_start[s + 1], len = b.lengths[s];
+    if (t < q0 || t >= q1) return w;
+  }
   w.seq = s;
   const int64_t pos = static_cast<int64_t>(len) - (q1 - static_cast<int64_t>(t));
-  const int64_t pi = pos >> b.ps_log2;
-  w.bad = pos < 0 || pi >= b.P;
-  if (!w.bad) {
-    w.pos = static_cast<int>(pos);
-    w.page = b.table[static_cast<int64_t>(s) * b.ld_table + pi];
-    w.bad = w.page < 0 || w.page >= b.pages;
-  }
+  w.bad = pos < 0 || pos >> b.ps_log2 >= b.P;
+  if (!w.bad) w.pos = static_cast<int>(pos);
   return w;
+}
+// The page of that position.
+__device__ __forceinline__ void kv4_page(const Kv4Batch& b, Kv4Where& w) {
+  if (w.seq < 0 || w.bad) return;
+  w.page = b.table[static_cast<int64_t>(w.seq) * b.ld_table + (w.pos >> b.ps_log2)];
+  w.bad = w.page < 0 || w.page >= b.pages;
 }
 
 struct Kv4AppendParams {
@@ -314,7 +328,7 @@ __device__ __forceinline__ bool kv4_quantise_fast(const float (&ya)[8], const fl
 // that could change a bit, so codes are those of the definition; v rows likewise, from exact values.
 // Bound by HBM at many rows: q in and out, k and v in, an eighth of that out as codes.
 template <typename T, int D, bool F32>
-__global__ void __launch_bounds__(256, 3) kv4_append_kernel(const Kv4AppendParams p) {
+__global__ void __launch_bounds__(256, 4) kv4_append_kernel(const Kv4AppendParams p) {
   using R = Kv4Rows<D>;
   constexpr int H = D / 2;
   const int t = blockIdx.x, hk = p.b.hk, rows = p.hq + 2 * hk;
@@ -339,18 +353,19 @@ __global__ void __launch_bounds__(256, 3) kv4_append_kernel(const Kv4AppendParam
     nb = *reinterpret_cast<const uint4*>(src + H);
   };
   load(r);
-  Kv4Where w = kv4_where(p.b, t);
+  Kv4Where w = kv4_position(p.b, t);
   if (w.seq >= 0 && !w.bad && w.pos >= p.table_rows) w.bad = true;
-  if (w.bad && threadIdx.x == 0) raise_status(kStatusBadIndex);
-  const bool real = w.seq >= 0 && !w.bad;
   Kv4Angles<T, F32> cos_a, cos_b, sin_a, sin_b;
-  if (real) {
+  if (w.seq >= 0 && !w.bad) {  // the angles travel while the page is looked up
     const int64_t at = static_cast<int64_t>(w.pos) * D + j0;
     cos_a.load(p.cos, at);
     cos_b.load(p.cos, at + H);
     sin_a.load(p.sin, at);
     sin_b.load(p.sin, at + H);
   }
+  kv4_page(p.b, w);
+  if (w.bad && threadIdx.x == 0) raise_status(kStatusBadIndex);
+  const bool real = w.seq >= 0 && !w.bad;
   const int64_t slot = w.pos & ((1 << p.b.ps_log2) - 1);
   auto store = [&](int row, const Kv4Row& y) {
     const bool is_k = row < p.hq + hk;
@@ -420,7 +435,8 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Batch b, T* k_ou
   const int t = blockIdx.x;
   const int r = blockIdx.y * R::kPerCta + threadIdx.x / R::kLanes;
   const int j0 = (threadIdx.x % R::kLanes) * 8;
-  const Kv4Where w = kv4_where(b, t);
+  Kv4Where w = kv4_position(b, t);
+  kv4_page(b, w);
   if (w.bad && threadIdx.x == 0) raise_status(kStatusBadIndex);
   if (r >= 2 * b.hk) return;
   const bool is_v = r >= b.hk;

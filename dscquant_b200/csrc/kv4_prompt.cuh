@@ -2,9 +2,11 @@
 // and the exponentials. See kv4_attention.cuh for the operator.
 //
 // A CTA takes 256 rows (tokens x query heads of one key head) of a sequence as two tiles of 128 and runs over the
-// keys they see, 128 at a time, with tcgen05 (kind::f16, M = 128):
-//   S_i = Q_i K^T   (TMEM, 128 columns each)     P_i = exp2(S_i - max) over S_i     O_i += P_i V   (TMEM)
-// While one tile's softmax runs, the other's products do. TMEM: S_0/P_0, S_1/P_1, O_0, O_1 = 512 columns.
+// keys they see, 64 at a time (128 to a stage of operands), with tcgen05 (kind::f16, M = 128):
+//   S_i = Q_i K^T   (TMEM, two buffers of 64 columns)     P_i = exp2(S_i - max) over S_i     O_i += P_i V   (TMEM)
+// The scores of the next 64 keys are made while a softmax runs (one buffer of 128 keys, whose softmax then waits for
+// its own products: 1.10 ms instead of 0.93 for 1000-1500-row chunks over 8k, 64/8 heads). TMEM: two tiles of two S/P
+// buffers, O_0, O_1 = 512 columns.
 //
 // Operands are fp16 whatever the cache's type. Codes become numbers on the way into shared memory, four warps, one key
 // a thread: a code in the low bits of an fp16 is the subnormal n 2^-24, so an AND and a fused multiply-add give
@@ -17,7 +19,8 @@
 // Keys no row may see (behind the end, on pages out of range) are zeros with their scores masked. A value row that is
 // not finite is zeros too and flagged; rows that see its key become NaN, the others must not.
 //
-// Warps 0-3, 4-7: softmax of tile 0 and 1 (a thread a row); 8-11: codes to operands; 12: MMA. All waits bounded.
+// Warps 0-3, 4-7: softmax of tile 0 and 1 (a thread a row); 8-11: codes to operands; 12, 13: the products of tile 0
+// and 1, a warp each so that neither waits for the other's weights. All waits bounded.
 #pragma once
 #include "kv4_decode.cuh"
 
@@ -28,7 +31,7 @@ struct Kv4PromptParams {
   int64_t min_rows;  // sequences with fewer rows * group than this are not this kernel's
 };
 
-constexpr int kKv4PromptThreads = 13 * 32;
+constexpr int kKv4PromptThreads = 14 * 32;
 constexpr int64_t kKv4AllRows = INT64_MAX;
 
 // x 2^e in two steps, for |e| up to 250.
@@ -78,8 +81,8 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
   uint8_t* vs = smem + 4 * C::kTile;   // [2]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 6 * C::kTile);
   uint64_t *qfull = bars, *kfull = bars + 1, *kempty = bars + 3, *vfull = bars + 5, *vempty = bars + 7;
-  uint64_t *sfull = bars + 9, *pfull = bars + 11, *ofull = bars + 15, *done = bars + 17;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+  uint64_t *sfull = bars + 9, *pfull = bars + 13, *odone = bars + 17, *done = bars + 19;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* item = reinterpret_cast<int*>(tmem_slot + 2);       // sequence, head, row tile
   int* kexp = item + 4;                                    // [2] exponents of the stages' scales
@@ -118,20 +121,27 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
         left -= __shfl_sync(0xffffffffu, upto, 31);
       }
     }
+    int halves = 1;
+    if (seq >= 0) {
+      const Kv4Seq r = kv4_seq<128, 256>(a, kKv4AllRows, seq);
+      halves = tile * 256 + 128 < r.n * a.group ? 2 : 1;
+    }
     if (lane == 0) {
       item[0] = seq, item[1] = head, item[2] = tile;
       mbar_init(qfull, 8);
       for (int i = 0; i < 2; ++i) {
         mbar_init(kfull + i, 4);
         mbar_init(vfull + i, 4);
-        mbar_init(kempty + i, 1);
-        mbar_init(vempty + i, 1);
-        mbar_init(sfull + i, 1);
+        mbar_init(kempty + i, halves);
+        mbar_init(vempty + i, halves);
+        mbar_init(sfull + 2 * i, 1);
+        mbar_init(sfull + 2 * i + 1, 1);
         mbar_init(pfull + 2 * i, 4);
         mbar_init(pfull + 2 * i + 1, 4);
-        mbar_init(ofull + i, 1);
+        mbar_init(odone + i, 1);
       }
       mbar_init(done, 1);
+      mbar_init(done + 1, 1);
       *abort_flag = 0;
       fence_mbar_init();
     }
@@ -150,7 +160,8 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
     const int halves = r0 + 128 < rows ? 2 : 1;
     // keys of row r: positions up to its own
     auto limit = [&](int r) { return min(sq.keys, sq.len - sq.n + a.row_token(r) + 1); };
-    const int tiles = max((limit(min(r0 + 256, rows) - 1) + 127) / 128, 1);
+    const int subs = max((limit(min(r0 + 256, rows) - 1) + 63) / 64, 1);  // 64 keys each
+    const int tiles = (subs + 1) / 2;
 
     if (warp < 8) {
       // ------------------------------------------------ queries, softmax, output: a thread a row
@@ -196,43 +207,41 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
         float m = -INFINITY, l[4] = {0.f, 0.f, 0.f, 0.f};
         int ev = -200;
         bool ok = true, nan = false;
-        for (int t = 0; t < tiles; ++t) {
-          const int s = t & 1;
-          const uint32_t ph = (t >> 1) & 1u;
-          ok = mbar_wait_spin(&sfull[half], t & 1u, abort_flag) && mbar_wait_spin(&vfull[s], ph, abort_flag);
+        for (int sub = 0; sub < subs; ++sub) {
+          const int t = sub >> 1, u = sub & 1, s = t & 1;
+          ok = mbar_wait(&sfull[2 * half + u], t & 1u, abort_flag) && mbar_wait(&vfull[s], (t >> 1) & 1u, abort_flag);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const int see = min(lim - t * 128, 128);  // columns this row sees
-          const uint32_t hidden = hide[s * 4] | hide[s * 4 + 1] | hide[s * 4 + 2] | hide[s * 4 + 3];
-          const uint32_t bad = poison[s * 4] | poison[s * 4 + 1] | poison[s * 4 + 2] | poison[s * 4 + 3];
-          const bool masked = __any_sync(0xffffffffu, see < 128) || hidden;
-          if (bad) {
+          const uint32_t at = s_at + u * 64;
+          uint32_t v[2][32];
+          tmem_ld32(at, v[0]);
+          tmem_ld32(at + 32, v[1]);
+          const int see = min(lim - sub * 64, 64);  // columns this row sees
+          const uint32_t hidden[2] = {hide[s * 4 + 2 * u], hide[s * 4 + 2 * u + 1]};
+          const uint32_t bad[2] = {poison[s * 4 + 2 * u], poison[s * 4 + 2 * u + 1]};
+          if (bad[0] | bad[1])
             for (int j = 0; j < see; ++j)
-              if ((poison[s * 4 + (j >> 5)] & ~hide[s * 4 + (j >> 5)]) >> (j & 31) & 1u) nan = true;
-          }
-          auto mask = [&](uint32_t (&v)[32], int c) {
-            const uint32_t h = hide[s * 4 + c];
-            if (!__any_sync(0xffffffffu, see < (c + 1) * 32 || h)) return;
+              if ((bad[j >> 5] & ~hidden[j >> 5]) >> (j & 31) & 1u) nan = true;
+          tmem_ld_wait();
+          // ---- the maximum
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (c * 32 + j >= see || (h >> j & 1u)) v[j] = 0xff800000u;
-          };
-          // ---- the tile's maximum
-          float mt = -INFINITY;
+          for (int c = 0; c < 2; ++c)
+            if (__any_sync(0xffffffffu, see < (c + 1) * 32 || hidden[c])) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32];
-            tmem_ld32(s_at + c * 32, v);
-            tmem_ld_wait();
-            if (masked) mask(v, c);
+              for (int j = 0; j < 32; ++j)
+                if (c * 32 + j >= see || (hidden[c] >> j & 1u)) v[c][j] = 0xff800000u;
+            }
+          float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int j = 0; j < 32; j += 2)
-              mt = fmaxf(fmaxf(mt, __uint_as_float(v[j])), __uint_as_float(v[j + 1]));
+          for (int j = 0; j < 32; j += 2) {
+            mx[0] = fmax3(mx[0], __uint_as_float(v[0][j]), __uint_as_float(v[0][j + 1]));
+            mx[1] = fmax3(mx[1], __uint_as_float(v[1][j]), __uint_as_float(v[1][j + 1]));
           }
           const float ce = times_pow2(c1, kexp[s]);
+          float mt = fmaxf(mx[0], mx[1]);
           mt = mt == -INFINITY ? mt : mt * ce;
           float f = 1.f;
           if (mt > m + 8.f || (m == -INFINITY && mt > m)) {
@@ -244,47 +253,47 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
           ev = e;
 #pragma unroll
           for (int j = 0; j < 4; ++j) l[j] *= f;
-          if (t > 0 && __any_sync(0xffffffffu, fo != 1.f)) {
-#pragma unroll
-            for (int c = 0; c < D; c += 32) {
-              uint32_t v[32];
-              tmem_ld32(o_at + c, v);
+          if (sub > 0 && __any_sync(0xffffffffu, fo != 1.f)) {
+            // the sums up to here must be complete (those before the last were when these scores came)
+            ok = mbar_wait(&odone[half], (sub - 1) & 1u, abort_flag);
+            if (!__all_sync(0xffffffffu, ok)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(o_at + c, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * fo);
-              tmem_st16(o_at + c, reinterpret_cast<const uint32_t(&)[16]>(v[0]));
-              tmem_st16(o_at + c + 16, reinterpret_cast<const uint32_t(&)[16]>(v[16]));
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * fo);
+              tmem_st16(o_at + c, o);
             }
           }
-          // ---- weights, over the scores they come from
-          // weights up to 2^15: small ones stay normal fp16 numbers down to 2^-21 of the largest
+          // ---- weights, over the scores they come from: up to 2^15, so small ones stay normal fp16 numbers down to
+          // 2^-21 of the largest
           const float base = m == -INFINITY ? 0.f : m - 7.f;
-          uint32_t v[2][32];
-          tmem_ld32(s_at, v[0]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            tmem_ld_wait();
-            if (c < 3) tmem_ld32(s_at + (c + 1) * 32, v[(c + 1) & 1]);
-            if (masked) mask(v[c & 1], c);
+          for (int c = 0; c < 2; ++c) {
             uint32_t w[16];
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
-              const float p0 = ex2(fmaf(__uint_as_float(v[c & 1][j]), ce, -base));
-              const float p1 = ex2(fmaf(__uint_as_float(v[c & 1][j + 1]), ce, -base));
+              const float p0 = ex2(fmaf(__uint_as_float(v[c][j]), ce, -base));
+              const float p1 = ex2(fmaf(__uint_as_float(v[c][j + 1]), ce, -base));
               l[j & 2] += p0;
               l[(j & 2) + 1] += p1;
               w[j / 2] = pack2<__half>(p0, p1);
             }
-            tmem_st16(s_at + c * 16, w);
-            if (c & 1) {
-              tmem_st_wait();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&pfull[2 * half + (c >> 1)]);
-            }
+            tmem_st16(at + c * 16, w);
           }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pfull[2 * half + u]);
         }
-        ok = ok && mbar_wait_spin(&ofull[half], 0, abort_flag);
+        if (ok && subs > 1) ok = mbar_wait(&odone[half], (subs - 2) & 1u, abort_flag);
+        ok = ok && mbar_wait(&odone[half], (subs - 1) & 1u, abort_flag);
         if (__all_sync(0xffffffffu, ok)) {
           tc_fence_after();
           const float sum = (l[0] + l[1]) + (l[2] + l[3]);
@@ -388,13 +397,13 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
         run = max(run, log2i(vm) + 7);
         if (lost) raise_status(kStatusBadIndex);
 
-        bool ok = t < 2 || mbar_wait_spin(&kempty[s], ph ^ 1u, abort_flag);
+        bool ok = t < 2 || mbar_wait(&kempty[s], ph ^ 1u, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) break;
         expand(ks + s * C::kTile, kc, kf, kx);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&kfull[s]);
-        ok = t < 2 || mbar_wait_spin(&vempty[s], ph ^ 1u, abort_flag);
+        ok = t < 2 || mbar_wait(&vempty[s], ph ^ 1u, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) break;
         expand(vs + s * C::kTile, vc, vf, run);
         if (lane == 0) {  // the tile's facts: its stage's last user read them before its values were multiplied
@@ -410,57 +419,55 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
       }
     } else {
       // ------------------------------------------------ MMA: the warp walks together, so addresses stay uniform
-      constexpr uint32_t id_qk = umma_idesc_f16(128, 128, false), id_pv = umma_idesc_f16(128, D, true);
+      constexpr uint32_t id_qk = umma_idesc_f16(128, 64, false), id_pv = umma_idesc_f16(128, D, true);
       const uint64_t q_desc = umma_desc_sw128(smem_u32(qs)), k_desc = umma_desc_sw128(smem_u32(ks));
       const uint64_t v_desc = umma_desc_sw128_mn_atoms(smem_u32(vs), C::kHalf);
-      auto scores = [&](int i, int s) {
-        const uint64_t qd = q_desc + static_cast<uint32_t>(i * C::kTile >> 4), kd = k_desc + static_cast<uint32_t>(s * C::kTile >> 4);
+      // S of tile i, keys 64 sub ..: into its buffer sub & 1
+      const int i = warp - 12;  // the tile
+      // S of keys 64 sub .. into its buffer sub & 1
+      auto scores = [&](int sub) {
+        const int s = (sub >> 1) & 1, u = sub & 1;
+        const uint64_t qd = q_desc + static_cast<uint32_t>(i * C::kTile >> 4);
+        const uint64_t kd = k_desc + static_cast<uint32_t>((s * C::kTile + u * 64 * 128) >> 4);
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t off = static_cast<uint32_t>((k >> 2) * C::kHalf + (k & 3) * 32) >> 4;
-            umma_f16_ss(tmem + i * 128, qd + off, kd + off, id_qk, k > 0 ? 1u : 0u);
+            umma_f16_ss(tmem + i * 128 + u * 64, qd + off, kd + off, id_qk, k > 0 ? 1u : 0u);
           }
-          umma_commit(&sfull[i]);
-          if (i + 1 == halves) umma_commit(&kempty[s]);
+          umma_commit(&sfull[2 * i + u]);
+          if (u == 1 || sub + 1 == subs) umma_commit(&kempty[s]);
         }
         __syncwarp();
       };
-      bool ok = mbar_wait_spin(qfull, 0, abort_flag) && mbar_wait_spin(&kfull[0], 0, abort_flag);
+      bool ok = i < halves && mbar_wait(qfull, 0, abort_flag) && mbar_wait(&kfull[0], 0, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
-      for (int i = 0; ok && i < halves; ++i) scores(i, 0);
-      for (int t = 0; ok && t < tiles; ++t) {
-        const int s = t & 1;
-        const uint64_t vd = v_desc + static_cast<uint32_t>(s * C::kTile >> 4);
-        for (int i = 0; ok && i < halves; ++i) {
-          if (i == 0) ok = mbar_wait_spin(&vfull[s], (t >> 1) & 1u, abort_flag);
-#pragma unroll
-          for (int part = 0; part < 2; ++part) {  // weights of 64 keys at a time
-            ok = ok && mbar_wait_spin(&pfull[2 * i + part], t & 1u, abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-#pragma unroll
-              for (int k = 4 * part; k < 4 * part + 4; ++k)
-                umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + k * 8, vd + (k * 2048 >> 4), id_pv,
-                            t > 0 || k > 0 ? 1u : 0u);
-              if (part == 1 && i + 1 == halves) umma_commit(&vempty[s]);
-              if (part == 1 && t + 1 == tiles) umma_commit(&ofull[i]);
-            }
-            __syncwarp();
-          }
-          if (ok && t + 1 < tiles) {
-            if (i == 0) ok = __all_sync(0xffffffffu, mbar_wait_spin(&kfull[s ^ 1], ((t + 1) >> 1) & 1u, abort_flag));
-            if (!ok) break;
-            tc_fence_after();
-            scores(i, s ^ 1);
-          }
+      for (int sub = 0; ok && sub < min(subs, 2); ++sub) scores(sub);
+      for (int sub = 0; ok && sub < subs; ++sub) {
+        const int t = sub >> 1, u = sub & 1, s = t & 1;
+        const uint64_t vd = v_desc + static_cast<uint32_t>((s * C::kTile + u * 64 * 128) >> 4);
+        if (u == 0) {
+          ok = mbar_wait(&vfull[s], (t >> 1) & 1u, abort_flag) &&
+               (sub + 2 >= subs || mbar_wait(&kfull[s ^ 1], ((t + 1) >> 1) & 1u, abort_flag));
         }
+        ok = ok && mbar_wait(&pfull[2 * i + u], t & 1u, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + u * 64 + k * 8, vd + (k * 2048 >> 4), id_pv,
+                        sub > 0 || k > 0 ? 1u : 0u);
+          umma_commit(&odone[i]);
+          if (u == 1 || sub + 1 == subs) umma_commit(&vempty[s]);
+        }
+        __syncwarp();
+        if (sub + 2 < subs) scores(sub + 2);
       }
-      if (elect_one()) umma_commit(done);
-      mbar_wait_spin(done, 0, nullptr);  // nothing is in flight when the memory goes
+      if (elect_one()) umma_commit(&done[i]);
+      mbar_wait(&done[i], 0, nullptr);  // nothing is in flight when the memory goes
     }
   }
   tc_fence_before();

@@ -65,7 +65,7 @@ constexpr int kLpCands = 1024;  // candidates kept
 // those not fit, or the row hold NaN or +inf, k passes for the next largest. Slices of a row meet through
 // distributed shared memory: their sums, and their k best each.
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads) logprob_rows(const LogprobParams p) {
+__global__ void __launch_bounds__(kLpThreads, 8) logprob_rows(const LogprobParams p) {
   constexpr int VE = 16 / sizeof(T);  // elements of a 16-byte load
   __shared__ uint64_t cand[kLpCands];
   __shared__ uint64_t best[64];  // this slice's top k
@@ -166,27 +166,32 @@ __global__ void __launch_bounds__(kLpThreads) logprob_rows(const LogprobParams p
 
   if (p.k) {
     const float tau = bound;
-    // f(value, index) over the thread's elements
-    auto mine_each = [&](auto f) {
-      for (int u = v0 + tid; u < v1; u += kLpThreads) {
-        float y[VE];
-        unpack(__ldg(xv + u), y);
+    // f(value, index) over the elements of the threads with `mine_in`; a warp goes over each such thread's loads
+    // together, one a lane, so looking again costs one trip to memory and not a chain of them
+    auto each_of = [&](bool mine_in, auto f) {
+      for (unsigned in = __ballot_sync(0xffffffffu, mine_in); in; in &= in - 1) {
+        const int first = v0 + warp * 32 + __ffs(in) - 1;
+#pragma unroll 1
+        for (int u = first + lane * kLpThreads; u < v1; u += 32 * kLpThreads) {
+          float y[VE];
+          unpack(__ldg(xv + u), y);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) f(y[e], head + u * VE + e);
+          for (int e = 0; e < VE; ++e) f(y[e], head + u * VE + e);
+        }
       }
-      if (lone >= 0) f(alone, lone);
+      if (mine_in && lone >= 0) f(alone, lone);
     };
     const bool plain = a.s == a.s;  // no NaN, no +inf
     int n = 0;
     bool rounds = !plain;
     if (plain) {
-      if (mine >= tau)
-        mine_each([&](float y, int i) {
-          if (y >= tau) {
-            const int at = atomicAdd(&found, 1);
-            if (at < kLpCands) cand[at] = logit_rank(y, i);
-          }
-        });
+      // (once there are too many, how many no longer matters)
+      each_of(mine >= tau, [&](float y, int i) {
+        if (y >= tau && *static_cast<volatile int*>(&found) <= kLpCands) {
+          const int at = atomicAdd(&found, 1);
+          if (at < kLpCands) cand[at] = logit_rank(y, i);
+        }
+      });
       __syncthreads();
       n = found;
       if (n > kLpCands) {
@@ -194,13 +199,12 @@ __global__ void __launch_bounds__(kLpThreads) logprob_rows(const LogprobParams p
         __syncthreads();
         if (tid == 0) found = 0;
         __syncthreads();
-        if (mine > tau)
-          mine_each([&](float y, int i) {
-            if (y > tau) {
-              const int at = atomicAdd(&found, 1);
-              if (at < kLpCands - 64) cand[at] = logit_rank(y, i);
-            }
-          });
+        each_of(mine > tau, [&](float y, int i) {
+          if (y > tau && *static_cast<volatile int*>(&found) <= kLpCands) {
+            const int at = atomicAdd(&found, 1);
+            if (at < kLpCands - 64) cand[at] = logit_rank(y, i);
+          }
+        });
         __syncthreads();
         n = found;
         rounds = n > kLpCands - 64;
@@ -225,7 +229,7 @@ __global__ void __launch_bounds__(kLpThreads) logprob_rows(const LogprobParams p
       uint64_t below = ~0ull;
       for (int i = 0; i < p.k; ++i) {
         uint64_t c = 0;
-        mine_each([&](float y, int j) {
+        each_of(true, [&](float y, int j) {
           const uint64_t z = logit_rank(y, j);
           if (z < below) c = umax64(c, z);
         });
