@@ -571,9 +571,9 @@ cudaError_t launch_kv4_attention(const dscq::Kv4AttnParams& a, int64_t max_q, vo
   if (rows <= 8) return launch_kv4_decode<T, D, 1>(a, all, ws, st);
   // Sequences of more than 64 rows go to the tensor-core kernel, when there can be enough of them to fill
   // a quarter of the GPU with CTAs of 256 rows.
-  const int64_t few = 64;
-  const int64_t ctas = (static_cast<int64_t>(a.T) * a.group / 256 + std::min<int64_t>(a.b.B, a.T)) * a.b.hk;
-  if (rows <= few || (static_cast<int64_t>(a.T) * a.group + 255) / 256 * a.b.hk < num_sms() / 4 || ctas >= (int64_t(1) << 31))
+  const int64_t few = 64, all_rows = static_cast<int64_t>(a.T) * a.group;
+  const int64_t ctas = (all_rows / 256 + std::min<int64_t>(a.b.B, all_rows / (few + 1))) * a.b.hk;
+  if (rows <= few || (all_rows + 255) / 256 * a.b.hk < num_sms() / 4 || ctas >= (int64_t(1) << 31))
     return launch_kv4_decode<T, D, 2>(a, all, ws, st);
   cudaError_t e = launch_kv4_decode<T, D, 2>(a, few, ws, st);
   if (e != cudaSuccess) return e;

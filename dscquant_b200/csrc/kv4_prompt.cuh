@@ -96,29 +96,40 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
     // this CTA's 256 rows; of a sequence the last ones, which see the most keys, first
     int64_t left = blockIdx.x;
     int seq = -1, head = 0, tile = 0;
-    for (int s0 = 0; s0 < a.b.B && seq < 0; s0 += 32) {
-      const int s = s0 + lane;
-      int64_t tiles = 0;
-      if (s < a.b.B) {
-        const Kv4Seq r = kv4_seq<128, 256>(a, kKv4AllRows, s);
-        tiles = static_cast<int64_t>(r.n) * a.group < p.min_rows ? 0 : r.blocks;
-      }
-      int64_t upto = tiles * a.b.hk;
+    auto tiles_of = [&](int s) -> int64_t {
+      const Kv4Seq r = kv4_seq<128, 256>(a, kKv4AllRows, s);
+      return static_cast<int64_t>(r.n) * a.group < p.min_rows ? 0 : static_cast<int64_t>(r.blocks) * a.b.hk;
+    };
+    auto scan32 = [&](int64_t v) {
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
+        const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
       }
-      const unsigned past = __ballot_sync(0xffffffffu, upto > left);
-      if (past) {
-        const int src = __ffs(past) - 1;
-        seq = s0 + src;
-        const int n = static_cast<int>(__shfl_sync(0xffffffffu, tiles, src));
-        const int at = static_cast<int>(left - __shfl_sync(0xffffffffu, upto - tiles * a.b.hk, src));
-        tile = n - 1 - at / a.b.hk;
-        head = at % a.b.hk;
-      } else {
-        left -= __shfl_sync(0xffffffffu, upto, 31);
+      return v;
+    };
+    // a lane adds up a stretch of sequences, then the warp looks through the stretch that holds this CTA
+    const int per = (a.b.B + 31) / 32;
+    int64_t mine = 0;
+#pragma unroll 4
+    for (int s = min(lane * per, a.b.B); s < min(lane * per + per, a.b.B); ++s) mine += tiles_of(s);
+    const int64_t upto = scan32(mine);
+    const unsigned past = __ballot_sync(0xffffffffu, upto > left);
+    if (past) {
+      const int who = __ffs(past) - 1, end = min(who * per + per, a.b.B);
+      left -= __shfl_sync(0xffffffffu, upto - mine, who);
+      for (int s0 = who * per; s0 < end && seq < 0; s0 += 32) {
+        const int64_t n = s0 + lane < end ? tiles_of(s0 + lane) : 0, sum = scan32(n);
+        const unsigned in = __ballot_sync(0xffffffffu, sum > left);
+        if (in) {
+          const int src = __ffs(in) - 1;
+          const int at = static_cast<int>(left - __shfl_sync(0xffffffffu, sum - n, src));
+          seq = s0 + src;
+          tile = static_cast<int>(__shfl_sync(0xffffffffu, n, src)) / a.b.hk - 1 - at / a.b.hk;
+          head = at % a.b.hk;
+        } else {
+          left -= __shfl_sync(0xffffffffu, sum, 31);
+        }
       }
     }
     int halves = 1;

@@ -252,6 +252,27 @@ def test_attention_prompts_with_awkward_cache(cuda_device, dtype):
     assert torch.equal(out[300:], want[300:]) and torch.isfinite(out).all()
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (96, 2)])
+def test_crowd(cuda_device, heads, kv_heads):
+    """More sequences than a warp or a CTA adds up at once, idle ones and a few prompts among them."""
+    from dscquant_b200 import ops
+
+    g = torch.Generator(device=cuda_device).manual_seed(13)
+    seqs = [(i % 3 != 0, 1 + i % 37) for i in range(1300)]
+    seqs[5], seqs[700], seqs[1290] = (150, 170), (90, 90), (70, 300)
+    bt = Batch([(int(n), L) for n, L in seqs], kv_heads, 64, 16, torch.bfloat16, cuda_device, pad=4)
+    bt.fill(g)
+    q = randn((bt.T, heads, 64), g, torch.bfloat16)
+    k, v = randn((bt.T, kv_heads, 64), g, torch.bfloat16), randn((bt.T, kv_heads, 64), g, torch.bfloat16)
+    cos, sin = tables(400, 64, torch.bfloat16, cuda_device)
+    before = snapshot(bt)
+    out = ops.kv4_append(bt.cache, q, k, v, cos, sin, *bt.where)
+    check_append(bt, q, k, v, cos, sin, out, before)
+    a = ops.kv4_attention(bt.cache, out, *bt.where)
+    check_attention(bt, out, a)
+    assert not a[bt.starts[-1]:].any()
+
+
 def test_attention_scale_strides_and_sharp_softmax(cuda_device):
     """Another scale, queries as a strided view, weights on single keys, keys far from zero."""
     from dscquant_b200 import ops
