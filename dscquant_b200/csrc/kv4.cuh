@@ -326,7 +326,10 @@ __device__ __forceinline__ bool kv4_quantise_fast(const float (&ya)[8], const fl
 // once the tokens alone fill the GPU). A group of D/16 lanes takes one row: q rows are rotated in 32 bits and
 // rounded once; k rows are rotated and quantised in 32 bits with a bound on the error, and again in 64 bits where
 // that could change a bit, so codes are those of the definition; v rows likewise, from exact values.
-// Bound by HBM at many rows: q in and out, k and v in, an eighth of that out as codes.
+// Bound by HBM at many rows: q in and out, k and v in, an eighth of that out as codes. Measured on a B200: 10158 tokens
+// of 32 + 32 + 32 heads of 128 in 112 us (3.4 TB/s, 0.53 of the copy rate; 101 us without the checks on the error), one
+// token in 5 us. 64 registers and four CTAs an SM beat 80 and three (129 us), despite a few spills: what is left is the
+// chain from a token's place in the batch to its angles.
 template <typename T, int D, bool F32>
 __global__ void __launch_bounds__(256, 4) kv4_append_kernel(const Kv4AppendParams p) {
   using R = Kv4Rows<D>;

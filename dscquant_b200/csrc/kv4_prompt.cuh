@@ -19,6 +19,11 @@
 // Keys no row may see (behind the end, on pages out of range) are zeros with their scores masked. A value row that is
 // not finite is zeros too and flagged; rows that see its key become NaN, the others must not.
 //
+// Measured on a B200: chunks of 1000 to 1500 rows over 8 to 10 thousand keys, 64 heads on 8: 926 us, 807 TFLOP/s (0.48 of
+// the cuBLAS rate); three prompts of 900 to 2048 tokens, 32 heads: 146 us. Without its products the kernel takes 912 us:
+// what binds is the softmax's own chain (read 64 scores, maximum, exponentials, write) and its handshakes, two
+// tiles' worth at a time; short prompts add 3 us of setting up and draining to each CTA's few tiles.
+//
 // Warps 0-3, 4-7: softmax of tile 0 and 1 (a thread a row); 8-11: codes to operands; 12, 13: the products of tile 0
 // and 1, a warp each so that neither waits for the other's weights. All waits bounded.
 #pragma once

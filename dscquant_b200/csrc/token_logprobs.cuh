@@ -64,6 +64,10 @@ constexpr int kLpCands = 1024;  // candidates kept
 // masked vocabulary) takes the strictly larger ones and the first k equal ones in index order; should even
 // those not fit, or the row hold NaN or +inf, k passes for the next largest. Slices of a row meet through
 // distributed shared memory: their sums, and their k best each.
+//
+// Measured on a B200: 4096 rows of 32000 bf16 logits in 57 us without alternatives (4.65 TB/s, 0.72 of the copy rate; the
+// exponentials alone need 30 us), 77 us with 20; one row 5 us (8 us with 5). Eight CTAs an SM (32 registers) hide the
+// trips to memory: 102 us at six with each thread going over its own logits again, 81 with its warp doing it.
 template <typename T>
 __global__ void __launch_bounds__(kLpThreads, 8) logprob_rows(const LogprobParams p) {
   constexpr int VE = 16 / sizeof(T);  // elements of a 16-byte load
