@@ -86,8 +86,8 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
   uint8_t* vs = smem + 4 * C::kTile;   // [2]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 6 * C::kTile);
   uint64_t *qfull = bars, *kfull = bars + 1, *kempty = bars + 3, *vfull = bars + 5, *vempty = bars + 7;
-  uint64_t *sfull = bars + 9, *pfull = bars + 13, *odone = bars + 17, *done = bars + 19;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
+  uint64_t *sfull = bars + 9, *pfull = bars + 13, *odone = bars + 17, *done = bars + 21;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* item = reinterpret_cast<int*>(tmem_slot + 2);       // sequence, head, row tile
   int* kexp = item + 4;                                    // [2] exponents of the stages' scales
@@ -154,7 +154,8 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
         mbar_init(sfull + 2 * i + 1, 1);
         mbar_init(pfull + 2 * i, 4);
         mbar_init(pfull + 2 * i + 1, 4);
-        mbar_init(odone + i, 1);
+        mbar_init(odone + 2 * i, 1);
+        mbar_init(odone + 2 * i + 1, 1);
       }
       mbar_init(done, 1);
       mbar_init(done + 1, 1);
@@ -235,13 +236,13 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
           uint32_t v[2][32];
           tmem_ld32(at, v[0]);
           tmem_ld32(at + 32, v[1]);
+          tmem_ld_wait();
           const int see = min(lim - sub * 64, 64);  // columns this row sees
           const uint32_t hidden[2] = {hide[s * 4 + 2 * u], hide[s * 4 + 2 * u + 1]};
           const uint32_t bad[2] = {poison[s * 4 + 2 * u], poison[s * 4 + 2 * u + 1]};
           if (bad[0] | bad[1])
             for (int j = 0; j < see; ++j)
               if ((bad[j >> 5] & ~hidden[j >> 5]) >> (j & 31) & 1u) nan = true;
-          tmem_ld_wait();
           // ---- the maximum
 #pragma unroll
           for (int c = 0; c < 2; ++c)
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
           for (int j = 0; j < 4; ++j) l[j] *= f;
           if (sub > 0 && __any_sync(0xffffffffu, fo != 1.f)) {
             // the sums up to here must be complete (those before the last were when these scores came)
-            ok = mbar_wait(&odone[half], (sub - 1) & 1u, abort_flag);
+            ok = mbar_wait(&odone[2 * half + (u ^ 1)], ((sub - 1) >> 1) & 1u, abort_flag);
             if (!__all_sync(0xffffffffu, ok)) {
               ok = false;
               break;
@@ -308,8 +309,9 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
           __syncwarp();
           if (lane == 0) mbar_arrive(&pfull[2 * half + u]);
         }
-        if (ok && subs > 1) ok = mbar_wait(&odone[half], (subs - 2) & 1u, abort_flag);
-        ok = ok && mbar_wait(&odone[half], (subs - 1) & 1u, abort_flag);
+        // A barrier for the sums of even and one for those of odd subs: its phase before the awaited one is then two subs
+        // old and surely over, and the one after it cannot come before this warp's next weights, so parity says which.
+        ok = ok && mbar_wait(&odone[2 * half + ((subs - 1) & 1)], ((subs - 1) >> 1) & 1u, abort_flag);
         if (__all_sync(0xffffffffu, ok)) {
           tc_fence_after();
           const float sum = (l[0] + l[1]) + (l[2] + l[3]);
@@ -476,7 +478,7 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
           for (int k = 0; k < 4; ++k)
             umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + u * 64 + k * 8, vd + (k * 2048 >> 4), id_pv,
                         sub > 0 || k > 0 ? 1u : 0u);
-          umma_commit(&odone[i]);
+          umma_commit(&odone[2 * i + u]);
           if (u == 1 || sub + 1 == subs) umma_commit(&vempty[s]);
         }
         __syncwarp();
