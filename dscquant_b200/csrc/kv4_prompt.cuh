@@ -5,7 +5,7 @@
 // keys they see, 64 at a time (128 to a stage of operands), with tcgen05 (kind::f16, M = 128):
 //   S_i = Q_i K^T   (TMEM, two buffers of 64 columns)     P_i = exp2(S_i - max) over S_i     O_i += P_i V   (TMEM)
 // The scores of the next 64 keys are made while a softmax runs (one buffer of 128 keys, whose softmax then waits for
-// its own products: 1.10 ms instead of 0.93 for 1000-1500-row chunks over 8k, 64/8 heads). TMEM: two tiles of two S/P
+// its own products: 1.10 ms instead of 0.98 for 1000-1500-row chunks over 8k, 64/8 heads). TMEM: two tiles of two S/P
 // buffers, O_0, O_1 = 512 columns.
 //
 // Operands are fp16 whatever the cache's type. Codes become numbers on the way into shared memory, four warps, one key
@@ -19,10 +19,11 @@
 // Keys no row may see (behind the end, on pages out of range) are zeros with their scores masked. A value row that is
 // not finite is zeros too and flagged; rows that see its key become NaN, the others must not.
 //
-// Measured on a B200: chunks of 1000 to 1500 rows over 8 to 10 thousand keys, 64 heads on 8: 926 us, 807 TFLOP/s (0.48 of
-// the cuBLAS rate); three prompts of 900 to 2048 tokens, 32 heads: 146 us. Without its products the kernel takes 912 us:
+// Measured on a B200: chunks of 1000 to 1500 rows over 8 to 10 thousand keys, 64 heads on 8: 933 us, 801 TFLOP/s (0.47 of
+// the cuBLAS rate); three prompts of 900 to 2048 tokens, 32 heads: 147 us. Without its products the kernel takes 912 us:
 // what binds is the softmax's own chain (read 64 scores, maximum, exponentials, write) and its handshakes, two
-// tiles' worth at a time; short prompts add 3 us of setting up and draining to each CTA's few tiles.
+// tiles' worth at a time; short prompts add 3 us of setting up and draining to each CTA's few tiles. One warp issuing both
+// tiles' products made the chunks 962 us.
 //
 // Warps 0-3, 4-7: softmax of tile 0 and 1 (a thread a row); 8-11: codes to operands; 12, 13: the products of tile 0
 // and 1, a warp each so that neither waits for the other's weights. All waits bounded.
