@@ -189,6 +189,8 @@ class LlamaW4A4:
         """Greedy continuation of each prompt (1-D ids, at least one): (ids [prompts, new_tokens], their log
         probabilities). The prompts run as one ragged step, the tokens behind the first through DecodeGraph."""
         counts = [len(p) for p in prompts]
+        if new_tokens < 1 or not counts or min(counts) < 1:
+            raise ValueError("generate needs at least one prompt, one id in each and one new token")
         used = [-(-(n + new_tokens) // page_size) for n in counts]
         caches = self.caches(sum(used), page_size)
         table = torch.full((len(prompts), max(used)), -1, dtype=torch.int32)
@@ -210,7 +212,7 @@ class LlamaW4A4:
         return torch.cat(ids[:new_tokens], 1), torch.cat(logprobs[:new_tokens], 1)
 
     def score(self, ids: torch.Tensor, top_k: int = 0) -> "ops.TokenLogprobs":
-        """Log probability of every token of ids [S] but the first given those before it, with the entropy and the
+        """Log probability of every token of ids [S >= 2] but the first given those before it, with the entropy and the
         top_k alternatives at each place; exp(-mean) of the log probabilities is the text's perplexity."""
         return ops.token_logprobs(self(ids)[:-1], ids[1:].contiguous(), top_k)
 

@@ -71,6 +71,14 @@ def test_generate_follows_eager_steps(model, cuda_device):
         rows = model.step(r.top_ids[:, 0], caches, table, torch.arange(4, device=cuda_device).int(), counts.int(), 1)
 
 
+def test_generate_refusals(model, cuda_device):
+    one = ids(3, cuda_device, 6)
+    for prompts, new in (([one], 0), ([], 4), ([one, one[:0]], 4)):
+        with pytest.raises(ValueError):
+            model.generate(prompts, new)
+    assert model.generate([one], 1)[0].shape == (1, 1)
+
+
 def test_score(model, cuda_device):
     x = ids(90, cuda_device, 4)
     r = model.score(x, top_k=3)
