@@ -230,12 +230,12 @@ __global__ void __launch_bounds__(kLpThreads, 8) logprob_rows(const LogprobParam
       }
     }
     if (rounds) {
-      uint64_t below = ~0ull;
+      uint64_t below = 0;
       for (int i = 0; i < p.k; ++i) {
         uint64_t c = 0;
         each_of(true, [&](float y, int j) {
           const uint64_t z = logit_rank(y, j);
-          if (z < below) c = umax64(c, z);
+          if (i == 0 || z < below) c = umax64(c, z);  // NaN at index 0 has the largest rank there is
         });
 #pragma unroll
         for (int o = 16; o; o >>= 1) c = umax64(c, __shfl_xor_sync(0xffffffffu, c, o));
