@@ -389,6 +389,7 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
       load(0);
       look(1);
       int run = -100;  // exponent of the largest value so far
+      bool ok = true;
       for (int t = 0; t < tiles; ++t) {
         const int s = t & 1;
         const uint32_t ph = (t >> 1) & 1u;
@@ -406,7 +407,8 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
         }
         if (lane == 0) tile_max[(s * 4 + part) * 2] = km, tile_max[(s * 4 + part) * 2 + 1] = vm;
         const unsigned gone = __ballot_sync(0xffffffffu, lost), ill = __ballot_sync(0xffffffffu, sick && have);
-        named_bar_sync(1, 128);
+        // a warp whose wait ran out still comes here, so that none of the others stays behind
+        if (!named_bar_and(1, 128, ok)) break;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           km = fmaxf(km, tile_max[(s * 4 + i) * 2]);
@@ -416,14 +418,14 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
         run = max(run, log2i(vm) + 7);
         if (lost) raise_status(kStatusBadIndex);
 
-        bool ok = t < 2 || mbar_wait(&kempty[s], ph ^ 1u, abort_flag);
-        if (!__all_sync(0xffffffffu, ok)) break;
+        ok = __all_sync(0xffffffffu, t < 2 || mbar_wait(&kempty[s], ph ^ 1u, abort_flag));
+        if (!ok) continue;
         expand(ks + s * C::kTile, kc, kf, kx);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&kfull[s]);
-        ok = t < 2 || mbar_wait(&vempty[s], ph ^ 1u, abort_flag);
-        if (!__all_sync(0xffffffffu, ok)) break;
+        ok = __all_sync(0xffffffffu, t < 2 || mbar_wait(&vempty[s], ph ^ 1u, abort_flag));
+        if (!ok) continue;
         expand(vs + s * C::kTile, vc, vf, run);
         if (lane == 0) {  // the tile's facts: its stage's last user read them before its values were multiplied
           hide[s * 4 + part] = gone;
