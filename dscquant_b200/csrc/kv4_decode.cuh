@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
     const int key0 = c.t * TILE;
     const bool masked = key0 + TILE > min_lim || (have & 0x80000000u);
 
-    // ---- the values' steps: F follows the largest
+    // ---- the values' steps, of either sign: F follows the largest
     uint32_t va[KB][2];
     float vmax = 0.f;
 #pragma unroll
@@ -525,7 +525,8 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
       poison = __any_sync(0xffffffffu, poison);
     }
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) vmax = fmax3(vmax, unpack2<T>(va[kb][0]).x, unpack2<T>(va[kb][1]).x);
+    for (int kb = 0; kb < KB; ++kb)
+      vmax = fmax3(vmax, fabsf(unpack2<T>(va[kb][0]).x), fabsf(unpack2<T>(va[kb][1]).x));
     float shrink = 1.f;
     if (__any_sync(0xffffffffu, vmax >= pow2f(vexp))) {
 #pragma unroll

@@ -1,0 +1,89 @@
+"""4-bit cache attention where cached rows differ by orders of magnitude or carry unusual numbers: rows a query does not
+see, or hardly weighs, must not cost it precision. Compared in 64 bits with bounds taken over the keys each row sees."""
+import pytest
+import torch
+
+from kv4_reference import Batch, pack, quantise, values
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.bfloat16, torch.float16]
+
+# (rows, cached tokens) of the sequences, heads, key heads: the few-row kernel, then the tensor-core one
+FEW = ([(4, 90), (1, 300), (6, 700)], 8, 2)
+MANY = ([(300, 300), (260, 400)], 32, 32)
+
+
+def randn(shape, gen, dtype, scale=1.0):
+    return (torch.randn(shape, generator=gen, device=gen.device) * scale).to(dtype)
+
+
+def reference(bt, q, scale=None):
+    """(out, tolerance) in float64. Per row and over the keys j it sees, p_j their weights: scores are off by 32-bit sums of
+    D products of |q| (15 |step| + |low|) and a rounding of each key to 11 bits, weights by that on both sides of their
+    normalisation; a weight (times up to 15 steps) and a value each round to 11 bits; weights under 2^-31 of the largest
+    contribution and elements under 2^-27 of their row may go."""
+    T, hq, D = q.shape
+    group, scale = hq // bt.kv_heads, D ** -0.5 if scale is None else scale
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(out)
+    for b, (n, L) in enumerate(bt.seqs):
+        if n == 0 or L <= 0:
+            continue
+        rows, pos = bt.rows(b)
+        pages, off = bt.slots(b, 0, L)
+        seen = torch.arange(L, device=q.device)[None] <= torch.tensor(list(pos), device=q.device)[:, None]
+        for h in range(bt.kv_heads):
+            ka, va = bt.cache.k_affine[pages, h, off].double(), bt.cache.v_affine[pages, h, off].double()
+            k = values(bt.cache.k_codes[pages, h, off], ka)
+            v = values(bt.cache.v_codes[pages, h, off], va)
+            for g in range(h * group, (h + 1) * group):
+                x = q[rows, g].double()
+                p = torch.softmax((x @ k.T * scale).masked_fill(~seen, -torch.inf), -1)
+                p = torch.where(seen.any(-1, keepdim=True), p, 0.0)
+                out[rows, g] = p @ v
+                size = x.abs().sum(-1, keepdim=True) * (15 * ka[:, 0].abs() + ka[:, 1].abs())
+                off_s = torch.where(seen, abs(scale) * (2.0 ** -23 * D * size + 2.0 ** -12 * (x.abs() @ k.abs().T)), 0.0)
+                off_s = off_s.amax(-1, keepdim=True) + 2.0 ** -20
+                row = v.abs().amax(-1)
+                tol[rows, g] = (2.1 * off_s + 2.0 ** -12) * (p @ v.abs()) + 2.0 ** -11 * (p @ (15 * va[:, :1].abs())) + \
+                    2.0 ** -27 * (p @ row)[:, None] + L * 2.0 ** -31 * (p * row).amax(-1, keepdim=True)
+    return out, tol + torch.finfo(bt.dtype).eps / 2 * (out.abs() + tol) + torch.finfo(bt.dtype).tiny
+
+
+def check(bt, q, out, scale=None):
+    ref, tol = reference(bt, q, scale)
+    err = (out.double() - ref).abs()
+    assert bool((err <= tol).all()), f"off by {float((err / tol).max()):.2f} of what is allowed"
+
+
+def put(bt, b, at, side, y):
+    """Cached rows of position `at` of sequence b: the quantised rows y [kv_heads, D]."""
+    pages, off = bt.slots(b, at, at + 1)
+    code, step, low = quantise(y[None].double(), bt.dtype)
+    getattr(bt.cache, side + "_codes")[pages, :, off] = pack(code)
+    getattr(bt.cache, side + "_affine")[pages, :, off] = torch.cat((step, low), -1).to(bt.dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("mix", [FEW, MANY], ids=["few", "many"])
+def test_steps_of_either_sign(cuda_device, dtype, D, mix):
+    """element = code * step + low holds for any pair: negative steps alone, and beside positive ones sixteen times smaller."""
+    from dscquant_b200 import ops
+
+    seqs, heads, kv_heads = mix
+    g = torch.Generator(device=cuda_device).manual_seed(21)
+    for signs in ("negative", "both"):
+        bt = Batch(seqs, kv_heads, D, 16, dtype, cuda_device)
+        bt.fill(g, v_offset=0.5)
+        for affine in (bt.cache.k_affine, bt.cache.v_affine):
+            a = torch.nan_to_num(affine.float())
+            flip = torch.ones_like(a[..., 0]) if signs == "negative" else \
+                (torch.rand(a[..., 0].shape, generator=g, device=cuda_device) < 0.3).float()
+            size = 1.0 if signs == "negative" else 1 + 15 * flip
+            # the row upside down: low becomes its largest element
+            affine[..., 1] = torch.where(flip > 0, a[..., 1] + 15 * a[..., 0] * size, a[..., 1]).to(dtype)
+            affine[..., 0] = torch.where(flip > 0, -a[..., 0] * size, a[..., 0]).to(dtype)
+        q = randn((bt.T, heads, D), g, dtype, 0.3)
+        check(bt, q, ops.kv4_attention(bt.cache, q, *bt.where))
