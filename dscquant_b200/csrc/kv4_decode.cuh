@@ -461,7 +461,9 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
             const float f = e & 1 ? qs * 0.0625f : qs;  // codes four bits up count sixteenfold
             qf[nt][w][e] = pack2<__half>(x[w][e] * f, x[w][e + 4] * f);
           }
-        const float sq = sum * qs * 0x1p-24f, cc = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2) * pow2f(24 - k);
+        // never 0: a masked score of -inf stays one
+        const float sq = sum * qs * 0x1p-24f;
+        const float cc = a.scale_log2 == 0.f ? 1.f : fmaxf(fabsf(a.scale_log2) * pow2f(24 - k), 0x1p-126f);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           sumq[nt][j] = __shfl_sync(0xffffffffu, sq, (2 * q + j) * 4);

@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
             mx[0] = fmax3(mx[0], __uint_as_float(v[0][j]), __uint_as_float(v[0][j + 1]));
             mx[1] = fmax3(mx[1], __uint_as_float(v[1][j]), __uint_as_float(v[1][j + 1]));
           }
-          const float ce = times_pow2(c1, kexp[s]);
+          const float ce = fmaxf(times_pow2(c1, kexp[s]), 0x1p-126f);  // never 0: a masked score of -inf stays one
           float mt = fmaxf(mx[0], mx[1]);
           mt = mt == -INFINITY ? mt : mt * ce;
           float f = 1.f;

@@ -87,3 +87,21 @@ def test_steps_of_either_sign(cuda_device, dtype, D, mix):
             affine[..., 0] = torch.where(flip > 0, -a[..., 0] * size, a[..., 0]).to(dtype)
         q = randn((bt.T, heads, D), g, dtype, 0.3)
         check(bt, q, ops.kv4_attention(bt.cache, q, *bt.where))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("mix", [FEW, MANY], ids=["few", "many"])
+def test_tiny_queries_keys_and_scales(cuda_device, dtype, mix):
+    """Scores that all but vanish weigh every visible key alike: zero or tiny keys, tiny queries, a tiny scale."""
+    from dscquant_b200 import ops
+
+    seqs, heads, kv_heads = mix
+    g = torch.Generator(device=cuda_device).manual_seed(22)
+    D = 64
+    small = 2.0 ** -60 if dtype is torch.bfloat16 else 2.0 ** -14
+    for keys, size, scale in ((0.0, small, None), (small, small, None), (1.0, 1.0, 1e-38), (1.0, small, 1e-30), (0.0, 1.0, -1e-38)):
+        bt = Batch(seqs, kv_heads, D, 16, dtype, cuda_device)
+        bt.fill(g, v_offset=0.5)
+        bt.cache.k_affine.copy_((torch.nan_to_num(bt.cache.k_affine.float()) * keys).to(dtype))
+        q = randn((bt.T, heads, D), g, dtype, size)
+        check(bt, q, ops.kv4_attention(bt.cache, q, *bt.where, scale=scale), scale)
