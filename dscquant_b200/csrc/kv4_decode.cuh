@@ -75,6 +75,11 @@ constexpr uint32_t kCode0 = 0x000F000Fu, kCode1 = 0x00F000F0u;  // two codes of 
 struct Kv4Seq {
   int q0, n, len, tiles, blocks;  // first row, rows, cached tokens (as given), tiles of a run, row blocks
   int keys;                       // cached tokens the page table can hold
+  // Keys row i sees: positions up to its own; none (0 or less) where that lies before the first or behind the page table.
+  __device__ __forceinline__ int sees(int i) const {
+    const int n_keys = len - n + i + 1;
+    return n_keys > keys ? 0 : n_keys;
+  }
 };
 
 template <int TILE, int RB>
@@ -469,8 +474,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
           sumq[nt][j] = __shfl_sync(0xffffffffu, sq, (2 * q + j) * 4);
           c1[nt][j] = __shfl_sync(0xffffffffu, cc, (2 * q + j) * 4);
           const int rr = r0 + nt * 8 + 2 * q + j;
-          // keys the row sees: positions up to its own
-          lim[nt][j] = rr < rows ? min(c.s.keys, c.s.len - c.s.n + a.row_token(rr) + 1) : 0;
+          lim[nt][j] = rr < rows ? c.s.sees(a.row_token(rr)) : 0;
           min_lim = min(min_lim, rr < rows ? lim[nt][j] : c.s.keys);
           max_lim = max(max_lim, lim[nt][j]);
           mx[nt][j] = -INFINITY;

@@ -176,9 +176,9 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
     const Kv4Seq sq = kv4_seq<128, 256>(a, kKv4AllRows, seq);
     const int rows = sq.n * a.group;
     const int halves = r0 + 128 < rows ? 2 : 1;
-    // keys of row r: positions up to its own
-    auto limit = [&](int r) { return min(sq.keys, sq.len - sq.n + a.row_token(r) + 1); };
-    const int subs = max((limit(min(r0 + 256, rows) - 1) + 63) / 64, 1);  // 64 keys each
+    // up to the last row's position; 64 keys each
+    const int reach = min(sq.keys, sq.len - sq.n + a.row_token(min(r0 + 256, rows) - 1) + 1);
+    const int subs = max((reach + 63) / 64, 1);
     const int tiles = (subs + 1) / 2;
 
     if (warp < 8) {
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
       if (live) {
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + half * 128 + lanes, o_at = tmem + 256 + half * 128 + lanes;
-        const int lim = real ? limit(r) : INT_MAX;  // a row of nothing masks nothing
+        const int lim = real ? sq.sees(tok) : INT_MAX;  // a row of nothing masks nothing
         float m = -INFINITY, l[4] = {0.f, 0.f, 0.f, 0.f};
         int ev = -200;
         bool ok = true, nan = false;

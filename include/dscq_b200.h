@@ -254,7 +254,8 @@ int dscq_silu_mul(const void* g, const void* u, int64_t n, void* y, void* stream
  * head_dim is 64 or 128, page_size a power of two from 16 to 1024. Codes, queries, keys, values, tables and
  * outputs are 16-byte aligned; strides are in elements and multiples of 8, the head dimension has stride 1.
  * What these arrays hold is checked on the device: a position before the first or behind max_pages pages, or a
- * page id outside [0, pages), is left out and raises bit 2 of dscq_device_status.
+ * page id outside [0, pages), is left out and raises bit 2 of dscq_device_status. (Attention gives zeros for rows at
+ * such positions; a position before the first, a row that sees no key, does not raise the bit there.)
  */
 typedef struct {
   void* k_codes;

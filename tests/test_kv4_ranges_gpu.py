@@ -105,3 +105,32 @@ def test_tiny_queries_keys_and_scales(cuda_device, dtype, mix):
         bt.cache.k_affine.copy_((torch.nan_to_num(bt.cache.k_affine.float()) * keys).to(dtype))
         q = randn((bt.T, heads, D), g, dtype, size)
         check(bt, q, ops.kv4_attention(bt.cache, q, *bt.where, scale=scale), scale)
+
+
+@pytest.mark.parametrize("mix", [FEW, MANY], ids=["few", "many"])
+def test_rows_behind_the_page_table_are_zero(cuda_device, mix):
+    """A length beyond what the page table holds: rows at positions behind it are left out (zero), the others stay."""
+    from dscquant_b200 import ops
+
+    seqs, heads, kv_heads = mix
+    g = torch.Generator(device=cuda_device).manual_seed(26)
+    bt = Batch(seqs, kv_heads, 64, 16, torch.bfloat16, cuda_device)
+    bt.fill(g)
+    q = randn((bt.T, heads, 64), g, torch.bfloat16)
+    n, L = seqs[-1]
+    room = 16 * bt.table.shape[1]
+    assert room - L < n or L == room
+    # the last sequence moves up until only its first two rows are inside
+    over = room - 2 + n
+    bt.table[-1, L // 16:] = bt.table[-1, 0]
+    bt.lengths[-1] = over
+    out = ops.kv4_attention(bt.cache, q, *bt.where)
+    assert ops.device_status(cuda_device) == 4
+    lo = bt.starts[-2]
+    assert not out[lo + 2:].any()
+    bt.lengths[-1] = room
+    bt.q_start[-1] = lo + 2
+    want = ops.kv4_attention(bt.cache, q[:lo + 2].contiguous(), *bt.where)
+    assert bool(out[lo:lo + 2].any())
+    err = (out[:lo + 2].float() - want.float()).abs()
+    assert bool((err <= 2.0 ** -6 * want.float().abs() + 2.0 ** -8).all())
