@@ -4,13 +4,14 @@
 // Mathematics. A 4-bit code n in the low bits of an fp16 number is the subnormal n 2^-24 (n 2^-20 four bits up), which
 // tensor cores multiply exactly; so an AND (and one shift for every other pair) makes two operands of two codes:
 //   q.k = step (q.n) + low sum(q)
-//   o   = sum_t P'_t n_t / F + sum_t p_t low_t,   P'_t = fp16(F p_t step_t)
+//   o   = sum_t P'_t n_t / F + sum_t p_t low_t,   P'_t = fp16(F p_t step_t), F of each row
 // and for f16 outputs, which would show the rounding of P' (4e-4 of the result), about the middle code, where it counts
 // a third: sum_t P'_t (n_t - 8) / F + sum_t p_t (low_t + 8 step_t), sum_t P'_t from one more product with ones.
 // No element is ever dequantised; step and low cost a few operations per key, not per element. Queries
 // enter as fp16, each row scaled by a power of two to the top of its range (exact but for elements 2^-29 below
-// the row's largest); F is a power of two that follows the largest step seen, so P' stays in range for any
-// step. Scores, softmax statistics and sums are 32-bit; only the weights P' are rounded, to 11 bits.
+// the row's largest); F is a power of two, a row's own, that falls when one of the row's weights times its step would
+// leave fp16: what the row does not see, or hardly weighs, costs it nothing. P' keeps 11 bits down to 2^-26 of the row's
+// largest contribution. Scores, softmax statistics and sums are 32-bit; only the weights P' are rounded.
 //
 // Fragments (mma.m16n8k16). Scores: A = 16 keys x 16 dims, B = 8 query rows; a lane's 32 dims (16 for D = 64)
 // of a key are one 16-byte load, any dim order works as long as the queries use the same. Output: A = 16
@@ -421,7 +422,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
   float o[NT][D / 16][4], ones[NT][4], mx[NT][2], l[NT][2], low[NT][2], sumq[NT][2], c1[NT][2];
   uint32_t qf[NT][W4][4];
   int lim[NT][2], min_lim = 0, max_lim = 0, t0 = 0;
-  int vexp = 0;  // every step of the values so far is below 2^vexp
+  float F[NT][2], cap = 0.f;  // F of the rows, powers of two; steps below cap cannot leave fp16 under any of them
   bool failed = false;
   int stage = 0;
   uint32_t parity = 0;
@@ -433,7 +434,6 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
       t0 = c.t;
       min_lim = INT_MAX;
       max_lim = 0;
-      vexp = -100;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int r = r0 + nt * 8 + g;
@@ -479,7 +479,9 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
           max_lim = max(max_lim, lim[nt][j]);
           mx[nt][j] = -INFINITY;
           l[nt][j] = low[nt][j] = 0.f;
+          F[nt][j] = lim[nt][j] > 0 ? 0x1p100f : 0x1p-100f;  // the first tile brings it down
         }
+        cap = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) ones[nt][e] = 0.f;
 #pragma unroll
@@ -509,7 +511,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
     const int key0 = c.t * TILE;
     const bool masked = key0 + TILE > min_lim || (have & 0x80000000u);
 
-    // ---- the values' steps, of either sign: F follows the largest
+    // ---- the values' steps, of either sign
     uint32_t va[KB][2];
     float vmax = 0.f;
 #pragma unroll
@@ -533,15 +535,6 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
       vmax = fmax3(vmax, fabsf(unpack2<T>(va[kb][0]).x), fabsf(unpack2<T>(va[kb][1]).x));
-    float shrink = 1.f;
-    if (__any_sync(0xffffffffu, vmax >= pow2f(vexp))) {
-#pragma unroll
-      for (int sh = 4; sh < 32; sh <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, sh));
-      const int e = min(log2i(vmax) + 1, 127);
-      shrink = e - vexp > 126 ? 0.f : pow2f(vexp - e);
-      vexp = e;
-    }
-    const float vf = vexp < -99 ? 0.f : pow2f(min(14 - vexp, 127));
 
     // ---- scores of the tile: s[nt][kb][.]: keys 16 kb + g (0, 1) and + 8 (2, 3), rows 2q (0, 2) and 2q + 1
     float s[NT][KB][4];
@@ -612,27 +605,59 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
         al[x] = mx[nt][x] == m ? 1.f : ex2(fmaf(mx[nt][x], c1[nt][x], -base[nt][x]));
         mx[nt][x] = m;
       }
-      if (__any_sync(0xffffffffu, al[0] * shrink != 1.f || al[1] * shrink != 1.f)) {
+      if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           l[nt][x] *= al[x];
           low[nt][x] *= al[x];
-          const float f = al[x] * shrink;
-          if constexpr (kMid) ones[nt][x] *= f;
+          if constexpr (kMid) ones[nt][x] *= al[x];
 #pragma unroll
           for (int d = 0; d < D / 16; ++d) {
-            o[nt][d][x] *= f;
-            o[nt][d][2 + x] *= f;
+            o[nt][d][x] *= al[x];
+            o[nt][d][2 + x] *= al[x];
           }
         }
       }
+    }
+
+    // ---- steps larger than any before under some row's F (seldom behind the first tile): rows whose weights they would
+    // take out of fp16 lower theirs, so that the largest is in [2^12, 2^13) and steps may still grow fourfold
+    if (__any_sync(0xffffffffu, vmax >= cap)) {
+      float top = 0.f;  // the largest F
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float w = 0.f;
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              w = fmaxf(w, ex2(fmaf(s[nt][kb][2 * j + x], c1[nt][x], -base[nt][x])) * fabsf(unpack2<T>(va[kb][j]).x));
+          w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, 4));
+          w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, 8));
+          w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, 16));
+          if (w * F[nt][x] >= 0x1p15f) {
+            const float less = pow2f(12 - log2i(w)), f = less / F[nt][x];
+            F[nt][x] = less;
+            if constexpr (kMid) ones[nt][x] *= f;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+              o[nt][d][x] *= f;
+              o[nt][d][2 + x] *= f;
+            }
+          }
+          top = fmaxf(top, F[nt][x]);
+        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      cap = 0x1p15f / top;  // a weight is at most 1 (2^-22 more): under 2^16
     }
 
     // ---- weights, and the output's products
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       const float2 v0 = unpack2<T>(va[kb][0]), v1 = unpack2<T>(va[kb][1]);
-      const float f0 = v0.x * vf, f1 = v1.x * vf;
       const float mid0 = kMid ? fmaf(8.f, v0.x, v0.y) : v0.y, mid1 = kMid ? fmaf(8.f, v1.x, v1.y) : v1.y;
       uint32_t bf[NT][2];
 #pragma unroll
@@ -643,7 +668,7 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
         for (int e = 0; e < 4; ++e) {
           pe[e] = ex2(fmaf(s[nt][kb][e], c1[nt][e & 1], -base[nt][e & 1]));
           l[nt][e & 1] += pe[e];
-          w[e] = pe[e] * (e < 2 ? f0 : f1);
+          w[e] = pe[e] * (e < 2 ? v0.x : v1.x) * F[nt][e & 1];
         }
         if (!poison) {
 #pragma unroll
@@ -706,7 +731,6 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
       const int slot = t0 > 0 ? 0 : 1;
       const bool last = i + 1 == count;  // the ring is free then, an earlier piece goes through the cache
       float* dst = last ? reinterpret_cast<float*>(ring) : first_all + warp * C::kPiece;
-      const float back = pow2f(vexp);  // 2^-24 of the codes and 2^(14 - vexp) of the weights, undone in two steps
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -719,11 +743,12 @@ __global__ void __launch_bounds__(C::WARPS * 32, 1) kv4_decode_kernel(const Kv4D
           }
           const int row = nt * 8 + 2 * q + x, rr = r0 + row;
           const float inv = whole ? (ls == 0.f ? 0.f : 1.f / ls) : 1.f;
+          const float back = 1.f / F[nt][x];  // and the codes' 2^-24 or 2^-20
           float y[D / 8];
 #pragma unroll
           for (int d = 0; d < D / 16; ++d) {
-            y[2 * d] = fmaf((o[nt][d][x] - ones[nt][x]) * 0x1p10f, back, lw) * inv;
-            y[2 * d + 1] = fmaf((o[nt][d][2 + x] - 16.f * ones[nt][x]) * 0x1p6f, back, lw) * inv;
+            y[2 * d] = fmaf((o[nt][d][x] - ones[nt][x]) * 0x1p24f, back, lw) * inv;
+            y[2 * d + 1] = fmaf((o[nt][d][2 + x] - 16.f * ones[nt][x]) * 0x1p20f, back, lw) * inv;
           }
           if (whole) {
             if (rr < rows) {

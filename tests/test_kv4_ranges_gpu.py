@@ -107,6 +107,62 @@ def test_tiny_queries_keys_and_scales(cuda_device, dtype, mix):
         check(bt, q, ops.kv4_attention(bt.cache, q, *bt.where, scale=scale), scale)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("mix", [FEW], ids=["few"])
+@pytest.mark.parametrize("log2", [12, 14, 40, 100])
+@pytest.mark.parametrize("side", ["k", "v"])
+def test_rows_do_not_feel_what_they_cannot_see(cuda_device, dtype, mix, log2, side):
+    """The newest tokens of each sequence far larger than all others: the rows before them are as exact as without them."""
+    from dscquant_b200 import ops
+
+    if dtype is torch.float16 and log2 > 14:
+        pytest.skip("beyond fp16")
+    seqs, heads, kv_heads = mix
+    g = torch.Generator(device=cuda_device).manual_seed(23)
+    D = 64
+    bt = Batch(seqs, kv_heads, D, 16, dtype, cuda_device)
+    bt.fill(g)
+    for b, (n, L) in enumerate(seqs):
+        # the largest of a sequence of many rows stands inside a block of keys that earlier rows see
+        for at in ({L - 1} if n < 64 else {L - 1, L - 70}):
+            put(bt, b, at, side, torch.randn(kv_heads, D, generator=g, device=cuda_device) * 2.0 ** log2)
+    q = randn((bt.T, heads, D), g, dtype)
+    out = ops.kv4_attention(bt.cache, q, *bt.where)
+    ref, tol = reference(bt, q)
+    before = torch.zeros(bt.T, dtype=torch.bool, device=cuda_device)
+    for b, (n, L) in enumerate(seqs):
+        last = L - 1 if n < 64 else L - 70
+        before[[bt.starts[b] + i for i, p in enumerate(range(L - n, L)) if p < last]] = True
+    assert int(before.sum()) > 5
+    err = (out.double() - ref).abs()[before] / tol[before]
+    assert bool((err <= 1).all()), f"off by {float(err.max()):.2f} of what is allowed"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("mix", [FEW], ids=["few"])
+@pytest.mark.parametrize("log2", [12, 14, 60])
+def test_large_values_of_no_weight(cuda_device, dtype, mix, log2):
+    """The first key's value is far larger than all others and its score far lower: it counts as much as its weight says."""
+    from dscquant_b200 import ops
+
+    if dtype is torch.float16 and log2 > 14:
+        pytest.skip("beyond fp16")
+    seqs, heads, kv_heads = mix
+    g = torch.Generator(device=cuda_device).manual_seed(24)
+    D = 64
+    bt = Batch(seqs, kv_heads, D, 16, dtype, cuda_device)
+    bt.fill(g)
+    low = torch.zeros(kv_heads, D, device=cuda_device)
+    low[:, 0] = -32.0 if log2 < 60 else -240.0
+    for b in range(len(seqs)):
+        put(bt, b, 0, "k", low)
+        put(bt, b, 0, "v", torch.randn(kv_heads, D, generator=g, device=cuda_device) * 2.0 ** log2)
+    q = randn((bt.T, heads, D), g, dtype)
+    q[..., 0] = 8
+    # the rows that see the first key alone have nothing else to be exact about
+    check(bt, q, ops.kv4_attention(bt.cache, q, *bt.where))
+
+
 @pytest.mark.parametrize("mix", [FEW, MANY], ids=["few", "many"])
 def test_rows_behind_the_page_table_are_zero(cuda_device, mix):
     """A length beyond what the page table holds: rows at positions behind it are left out (zero), the others stay."""
