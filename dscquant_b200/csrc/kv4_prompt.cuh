@@ -11,10 +11,19 @@
 // Operands are fp16 whatever the cache's type. Codes become numbers on the way into shared memory, four warps, one key
 // a thread: a code in the low bits of an fp16 is the subnormal n 2^-24, so an AND and a fused multiply-add give
 // round(n step' + low') for two elements, with (step', low') scaled by a power of two that puts the tile's largest
-// value under 2^-6 (for values: the largest so far; sums already made follow). That rounds keys and values to 11
-// bits; queries, scaled by a power of two a row, are exact. Scores, statistics and sums are 32-bit. Weights are
-// fp16 (11 bits, 2^-21 of the largest and more), relative to a running maximum that only moves when it would be passed by 2^8:
-// then the row's sums in TMEM are scaled, by the warps that own them.
+// element under 2^-6. That rounds keys and values to 11 bits; queries, scaled by a power of two a row, are exact. Scores,
+// statistics and sums are 32-bit.
+//
+// What a row does not see, or hardly weighs, must not cost it bits. With s_j the score of key j and v_j = V_j 2^(E_j) its
+// scaled value row, the weights handed to the product are W_j = fp16(2^(T_j - M)), T_j = s_j + E_j, M a running maximum of
+// the T_j that the row sees, and
+//   out = 2^M sum W_j V_j / sum 2^(s_j).
+// E_j is the tile's exponent, but a key whose largest element is under 1/16 of the tile's has its own (and keys
+// their own scale likewise), so that fp16 keeps 2^-13 of every row's largest element at least. Tiles with such keys, and those whose exponent is 20 below an earlier one, so that
+// the sum of the 2^(s_j) cannot be had from the weights in 32 bits, are marked wide and take a slower path. M is a whole
+// number and only moves when it would be passed by 2^8; then the row's sums in TMEM are scaled, by the warps that own
+// them. Weights keep 11 bits down to 2^-21 of the largest. (The slower path is a loop over TMEM: a second copy of the
+// unrolled one cost the other tiles 9% for its length alone.)
 //
 // Keys no row may see (behind the end, on pages out of range) are zeros with their scores masked. A value row that is
 // not finite is zeros too and flagged; rows that see its key become NaN, the others must not.
@@ -69,11 +78,24 @@ __device__ __forceinline__ bool elect_one() {
   return is != 0;
 }
 
+// 32 lanes x 32 bit, 8 consecutive columns per thread.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
 template <int D>
 struct Kv4PromptConfig {
   static constexpr int kHalf = 128 * 128;               // 128 rows of 64 fp16, 128-byte swizzled
   static constexpr int kTile = D / 64 * kHalf;          // an operand of 128 rows
-  static constexpr int kSmem = 1024 + 6 * kTile + 1024; // Q_0, Q_1, two stages of K and of V; barriers, tile facts
+  static constexpr int kSmem = 1024 + 6 * kTile + 2048; // Q_0, Q_1, two stages of K and of V; barriers, tile facts
 };
 
 template <typename T, int D>
@@ -95,7 +117,9 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
   int* vexp = kexp + 2;
   uint32_t* hide = reinterpret_cast<uint32_t*>(vexp + 2);  // [2][4] keys on pages out of range
   uint32_t* poison = hide + 8;                             // [2][4] keys whose values are not finite
-  float* tile_max = reinterpret_cast<float*>(poison + 8);  // [2][4][2]
+  uint32_t* wide = poison + 8;                             // [2][4] keys with scales of their own
+  uint32_t* shift = wide + 8;                              // [2][128] their exponents below the tile's: keys | values << 16
+  float* tile_max = reinterpret_cast<float*>(shift + 256); // [2][4][2]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (warp == 12) {
@@ -222,8 +246,8 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + half * 128 + lanes, o_at = tmem + 256 + half * 128 + lanes;
         const int lim = real ? sq.sees(tok) : INT_MAX;  // a row of nothing masks nothing
-        float m = -INFINITY, l[4] = {0.f, 0.f, 0.f, 0.f};
-        int ev = -200;
+        float m = -INFINITY, l = 0.f;  // M, a whole number
+        int unit = -1000;              // sum 2^(s_j) = l 2^unit
         bool ok = true, nan = false;
         for (int sub = 0; sub < subs; ++sub) {
           const int t = sub >> 1, u = sub & 1, s = t & 1;
@@ -234,13 +258,45 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
           }
           tc_fence_after();
           const uint32_t at = s_at + u * 64;
+          const int see = min(lim - sub * 64, 64);  // columns this row sees
+          const uint32_t hidden[2] = {hide[s * 4 + 2 * u], hide[s * 4 + 2 * u + 1]};
+          const uint32_t bad[2] = {poison[s * 4 + 2 * u], poison[s * 4 + 2 * u + 1]};
+          const float ev = static_cast<float>(vexp[s]);
+          float ce = fmaxf(times_pow2(c1, kexp[s]), 0x1p-126f);  // never 0: a masked score of -inf stays one
+          float own_sum = 0.f, own_top = -INFINITY;
+          const bool own = (wide[s * 4 + 2 * u] | wide[s * 4 + 2 * u + 1]) != 0;
+          if (own) {
+            // keys with exponents of their own: T_j - E takes the place of their scores, and the s_j are summed up here
+            const uint32_t* sh = shift + s * 128 + u * 64;
+#pragma unroll 1
+            for (int c = 0; c < 64; c += 8) {
+              uint32_t x[8];
+              tmem_ld8(at + c, x);
+              tmem_ld_wait();
+              float top = own_top, y[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const uint32_t e = sh[c + j];
+                const bool seen = c + j < see && !(hidden[c >> 5] >> ((c & 31) + j) & 1u);
+                y[j] = times_pow2(__uint_as_float(x[j]), -static_cast<int>(e & 0xffffu)) * ce;
+                x[j] = __float_as_uint(y[j] - static_cast<float>(e >> 16));
+                y[j] = seen ? y[j] : -INFINITY;
+                top = fmaxf(top, y[j]);
+              }
+              tmem_st8(at + c, x);
+              top = top == -INFINITY ? top : ceilf(top);
+              own_sum *= top == own_top ? 1.f : ex2(own_top - top);
+              own_top = top;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) own_sum += y[j] == -INFINITY ? 0.f : ex2(y[j] - top);
+            }
+            tmem_st_wait();
+            ce = 1.f;
+          }
           uint32_t v[2][32];
           tmem_ld32(at, v[0]);
           tmem_ld32(at + 32, v[1]);
           tmem_ld_wait();
-          const int see = min(lim - sub * 64, 64);  // columns this row sees
-          const uint32_t hidden[2] = {hide[s * 4 + 2 * u], hide[s * 4 + 2 * u + 1]};
-          const uint32_t bad[2] = {poison[s * 4 + 2 * u], poison[s * 4 + 2 * u + 1]};
           if (bad[0] | bad[1])
             for (int j = 0; j < see; ++j)
               if ((bad[j >> 5] & ~hidden[j >> 5]) >> (j & 31) & 1u) nan = true;
@@ -258,20 +314,14 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
             mx[0] = fmax3(mx[0], __uint_as_float(v[0][j]), __uint_as_float(v[0][j + 1]));
             mx[1] = fmax3(mx[1], __uint_as_float(v[1][j]), __uint_as_float(v[1][j + 1]));
           }
-          const float ce = fmaxf(times_pow2(c1, kexp[s]), 0x1p-126f);  // never 0: a masked score of -inf stays one
           float mt = fmaxf(mx[0], mx[1]);
-          mt = mt == -INFINITY ? mt : mt * ce;
+          mt = mt == -INFINITY ? mt : fmaf(mt, ce, ev);
           float f = 1.f;
           if (mt > m + 8.f || (m == -INFINITY && mt > m)) {
-            f = ex2(m - mt);
-            m = mt;
+            f = pow2f(static_cast<int>(fmaxf(m - ceilf(mt), -126.f)));
+            m = ceilf(mt);
           }
-          const int e = vexp[s];
-          const float fo = e == ev ? f : f * pow2f(max(ev - e, -126));  // e never falls
-          ev = e;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) l[j] *= f;
-          if (sub > 0 && __any_sync(0xffffffffu, fo != 1.f)) {
+          if (sub > 0 && __any_sync(0xffffffffu, f != 1.f)) {
             // the sums up to here must be complete (those before the last were when these scores came)
             ok = mbar_wait(&odone[2 * half + (u ^ 1)], ((sub - 1) >> 1) & 1u, abort_flag);
             if (!__all_sync(0xffffffffu, ok)) {
@@ -285,13 +335,14 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
               tmem_ld16(o_at + c, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * fo);
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
               tmem_st16(o_at + c, o);
             }
           }
           // ---- weights, over the scores they come from: up to 2^15, so small ones stay normal fp16 numbers down to
           // 2^-21 of the largest
-          const float base = m == -INFINITY ? 0.f : m - 7.f;
+          const float base = m == -INFINITY ? 0.f : m - 7.f - ev;
+          float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             uint32_t w[16];
@@ -299,15 +350,23 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
             for (int j = 0; j < 32; j += 2) {
               const float p0 = ex2(fmaf(__uint_as_float(v[c][j]), ce, -base));
               const float p1 = ex2(fmaf(__uint_as_float(v[c][j + 1]), ce, -base));
-              l[j & 2] += p0;
-              l[(j & 2) + 1] += p1;
+              sums[j & 2] += p0;
+              sums[(j & 2) + 1] += p1;
               w[j / 2] = pack2<__half>(p0, p1);
             }
             tmem_st16(at + c * 16, w);
           }
+          // ---- the sum of 2^(s_j) is that of 2^(T_j - M + 7) in units of 2^base, where the keys share an exponent
+          const float sum = own ? own_sum : (sums[0] + sums[1]) + (sums[2] + sums[3]);
+          int in = static_cast<int>(own ? own_top : base);
+          if (mt == -INFINITY) in = unit;  // (a sum over nothing, 0 or NaN)
+          const int to = max(unit, in);
+          l = fmaf(l, pow2f(max(unit - to, -126)), sum * pow2f(max(in - to, -126)));
+          unit = to;
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
+          // from here on the tile's facts may give way to those of the next tile in this stage
           if (lane == 0) mbar_arrive(&pfull[2 * half + u]);
         }
         // A barrier for the sums of even and one for those of odd subs: its phase before the awaited one is then two subs
@@ -315,8 +374,8 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
         ok = ok && mbar_wait(&odone[2 * half + ((subs - 1) & 1)], ((subs - 1) >> 1) & 1u, abort_flag);
         if (__all_sync(0xffffffffu, ok)) {
           tc_fence_after();
-          const float sum = (l[0] + l[1]) + (l[2] + l[3]);
-          const float inv = nan ? __int_as_float(0x7fc00000) : sum == 0.f ? 0.f : 1.f / sum;
+          const float inv = nan ? __int_as_float(0x7fc00000) : l == 0.f ? 0.f : 1.f / l;
+          const int ev = m == -INFINITY ? 0 : min(max(static_cast<int>(m) - 7 - unit, -250), 250);
           T* out = static_cast<T*>(a.out) + ((sq.q0 + static_cast<int64_t>(tok)) * a.hq + hd) * D;
 #pragma unroll
           for (int c = 0; c < D; c += 32) {
@@ -388,8 +447,10 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
       look(0);
       load(0);
       look(1);
-      int run = -100;  // exponent of the largest value so far
       bool ok = true;
+      int run = -1000;  // the largest exponent of values so far
+      // the exponent that puts a largest element of x under 2^-6
+      auto exponent = [](float x) { return log2i(x) + 7; };
       for (int t = 0; t < tiles; ++t) {
         const int s = t & 1;
         const uint32_t ph = (t >> 1) & 1u;
@@ -400,6 +461,7 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
         float vm = fmaxf(fabsf(vf.y), fabsf(fmaf(15.f, vf.x, vf.y)));
         if (!(km < INFINITY)) km = 0.f;
         if (!(vm < INFINITY)) vm = 0x1.fffffep127f;
+        const float kown = km, vown = vm;
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
           km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, o));
@@ -414,23 +476,29 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
           km = fmaxf(km, tile_max[(s * 4 + i) * 2]);
           vm = fmaxf(vm, tile_max[(s * 4 + i) * 2 + 1]);
         }
-        const int kx = max(log2i(km), -100) + 7;  // the largest goes under 2^-6
-        run = max(run, log2i(vm) + 7);
+        const int kx = exponent(km), vx = exponent(vm);
+        // keys far below the tile's largest have exponents of their own (zeros fit any)
+        auto apart = [&](float x, int tile) { return x > 0.f && tile - exponent(x) > 4 ? tile - exponent(x) : 0; };
+        const int ksh = apart(kown, kx), vsh = apart(vown, vx);
+        run = max(run, vx);
+        const unsigned far = __ballot_sync(0xffffffffu, ksh | vsh || vx < run - 20);
         if (lost) raise_status(kStatusBadIndex);
 
         ok = __all_sync(0xffffffffu, t < 2 || mbar_wait(&kempty[s], ph ^ 1u, abort_flag));
         if (!ok) continue;
-        expand(ks + s * C::kTile, kc, kf, kx);
+        expand(ks + s * C::kTile, kc, kf, kx - ksh);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&kfull[s]);
         ok = __all_sync(0xffffffffu, t < 2 || mbar_wait(&vempty[s], ph ^ 1u, abort_flag));
         if (!ok) continue;
-        expand(vs + s * C::kTile, vc, vf, run);
+        expand(vs + s * C::kTile, vc, vf, vx - vsh);
+        shift[s * 128 + key] = static_cast<uint32_t>(ksh) | static_cast<uint32_t>(vsh) << 16;
         if (lane == 0) {  // the tile's facts: its stage's last user read them before its values were multiplied
           hide[s * 4 + part] = gone;
           poison[s * 4 + part] = ill;
-          if (part == 0) kexp[s] = kx, vexp[s] = run;
+          wide[s * 4 + part] = far;
+          if (part == 0) kexp[s] = kx, vexp[s] = vx;
         }
         fence_proxy_async_smem();
         __syncwarp();

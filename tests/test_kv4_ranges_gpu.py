@@ -108,7 +108,7 @@ def test_tiny_queries_keys_and_scales(cuda_device, dtype, mix):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("mix", [FEW], ids=["few"])
+@pytest.mark.parametrize("mix", [FEW, MANY], ids=["few", "many"])
 @pytest.mark.parametrize("log2", [12, 14, 40, 100])
 @pytest.mark.parametrize("side", ["k", "v"])
 def test_rows_do_not_feel_what_they_cannot_see(cuda_device, dtype, mix, log2, side):
@@ -139,7 +139,7 @@ def test_rows_do_not_feel_what_they_cannot_see(cuda_device, dtype, mix, log2, si
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("mix", [FEW], ids=["few"])
+@pytest.mark.parametrize("mix", [FEW, MANY], ids=["few", "many"])
 @pytest.mark.parametrize("log2", [12, 14, 60])
 def test_large_values_of_no_weight(cuda_device, dtype, mix, log2):
     """The first key's value is far larger than all others and its score far lower: it counts as much as its weight says."""
