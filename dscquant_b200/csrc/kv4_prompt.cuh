@@ -13,14 +13,18 @@
 // round(n step' + low') for two elements, with (step', low') scaled by a power of two that puts the tile's largest
 // element under 2^-6. That rounds keys and values to 11 bits; queries, scaled by a power of two a row, are exact. Scores,
 // statistics and sums are 32-bit.
+// For f16, whose outputs would show that rounding (7e-4 of the result against 64 bits instead of 3e-4), keys and values are
+// made in 32 bits and split into two fp16 parts, 21 bits, each multiplied: twice the products, and stages of 64 keys
+// instead of 128 for the same memory. The weights' rounding is the one that stays.
 //
 // What a row does not see, or hardly weighs, must not cost it bits. With s_j the score of key j and v_j = V_j 2^(E_j) its
 // scaled value row, the weights handed to the product are W_j = fp16(2^(T_j - M)), T_j = s_j + E_j, M a running maximum of
 // the T_j that the row sees, and
 //   out = 2^M sum W_j V_j / sum 2^(s_j).
-// E_j is the tile's exponent, but a key whose largest element is under 1/16 of the tile's has its own (and keys
+// E_j is the tile's exponent, but for bf16 a key whose largest element is under 1/16 of the tile's has its own (and keys
 // their own scale likewise), so that fp16 keeps 2^-13 of every row's largest element at least. Tiles with such keys, and those whose exponent is 20 below an earlier one, so that
-// the sum of the 2^(s_j) cannot be had from the weights in 32 bits, are marked wide and take a slower path. M is a whole
+// the sum of the 2^(s_j) cannot be had from the weights in 32 bits, are marked wide and take a slower path. (All of f16's
+// range fits two parts under one scale: the largest element goes under 2^15, and 2^-40 of it stays.) M is a whole
 // number and only moves when it would be passed by 2^8; then the row's sums in TMEM are scaled, by the warps that own
 // them. Weights keep 11 bits down to 2^-21 of the largest. (The slower path is a loop over TMEM: a second copy of the
 // unrolled one cost the other tiles 9% for its length alone.)
@@ -34,7 +38,8 @@
 // tiles' worth at a time; short prompts add 3 us of setting up and draining to each CTA's few tiles. One warp issuing both
 // tiles' products made the chunks 962 us.
 //
-// Warps 0-3, 4-7: softmax of tile 0 and 1 (a thread a row); 8-11: codes to operands; 12, 13: the products of tile 0
+// Warps 0-3, 4-7: softmax of tile 0 and 1 (a thread a row); 8-11: codes to operands (split: 8, 9 the even, 10, 11 the odd
+// 64 keys, independently); 12, 13: the products of tile 0
 // and 1, a warp each so that neither waits for the other's weights. All waits bounded.
 #pragma once
 #include "kv4_decode.cuh"
@@ -101,11 +106,12 @@ struct Kv4PromptConfig {
 template <typename T, int D>
 __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const Kv4PromptParams p) {
   using C = Kv4PromptConfig<D>;
+  constexpr bool kSplit = std::is_same<T, __half>::value;
   const Kv4AttnParams& a = p.a;
   extern __shared__ uint8_t kv4_prompt_smem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kv4_prompt_smem) + 1023) & ~uintptr_t(1023));
   uint8_t* qs = smem;                  // [2]
-  uint8_t* ks = smem + 2 * C::kTile;   // [2]
+  uint8_t* ks = smem + 2 * C::kTile;   // [2] tiles, or the two parts of one
   uint8_t* vs = smem + 4 * C::kTile;   // [2]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 6 * C::kTile);
   uint64_t *qfull = bars, *kfull = bars + 1, *kempty = bars + 3, *vfull = bars + 5, *vempty = bars + 7;
@@ -113,14 +119,17 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* item = reinterpret_cast<int*>(tmem_slot + 2);       // sequence, head, row tile
-  int* kexp = item + 4;                                    // [2] exponents of the stages' scales
-  int* vexp = kexp + 2;
-  uint32_t* hide = reinterpret_cast<uint32_t*>(vexp + 2);  // [2][4] keys on pages out of range
+  int* kexp = item + 4;                                    // [2][2] exponents of the scales of 64 keys
+  int* vexp = kexp + 4;
+  uint32_t* hide = reinterpret_cast<uint32_t*>(vexp + 4);  // [2][4] keys on pages out of range
   uint32_t* poison = hide + 8;                             // [2][4] keys whose values are not finite
   uint32_t* wide = poison + 8;                             // [2][4] keys with scales of their own
   uint32_t* shift = wide + 8;                              // [2][128] their exponents below the tile's: keys | values << 16
   float* tile_max = reinterpret_cast<float*>(shift + 256); // [2][4][2]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // A stage of operands holds 128 keys, split 64: where those of 64 keys `sub` go, and how often it was filled before.
+  auto stage_of = [](int sub) { return (kSplit ? sub : sub >> 1) & 1; };
+  auto use_of = [](int sub) { return static_cast<uint32_t>(kSplit ? sub >> 1 : sub >> 2); };
 
   if (warp == 12) {
     // this CTA's 256 rows; of a sequence the last ones, which see the most keys, first
@@ -171,8 +180,8 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
       item[0] = seq, item[1] = head, item[2] = tile;
       mbar_init(qfull, 8);
       for (int i = 0; i < 2; ++i) {
-        mbar_init(kfull + i, 4);
-        mbar_init(vfull + i, 4);
+        mbar_init(kfull + i, kSplit ? 2 : 4);
+        mbar_init(vfull + i, kSplit ? 2 : 4);
         mbar_init(kempty + i, halves);
         mbar_init(vempty + i, halves);
         mbar_init(sfull + 2 * i, 1);
@@ -251,7 +260,8 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
         bool ok = true, nan = false;
         for (int sub = 0; sub < subs; ++sub) {
           const int t = sub >> 1, u = sub & 1, s = t & 1;
-          ok = mbar_wait(&sfull[2 * half + u], t & 1u, abort_flag) && mbar_wait(&vfull[s], (t >> 1) & 1u, abort_flag);
+          ok = mbar_wait(&sfull[2 * half + u], t & 1u, abort_flag) &&
+               mbar_wait(&vfull[stage_of(sub)], use_of(sub) & 1u, abort_flag);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
@@ -261,10 +271,10 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
           const int see = min(lim - sub * 64, 64);  // columns this row sees
           const uint32_t hidden[2] = {hide[s * 4 + 2 * u], hide[s * 4 + 2 * u + 1]};
           const uint32_t bad[2] = {poison[s * 4 + 2 * u], poison[s * 4 + 2 * u + 1]};
-          const float ev = static_cast<float>(vexp[s]);
-          float ce = fmaxf(times_pow2(c1, kexp[s]), 0x1p-126f);  // never 0: a masked score of -inf stays one
+          const float ev = static_cast<float>(vexp[s * 2 + u]);
+          float ce = fmaxf(times_pow2(c1, kexp[s * 2 + u]), 0x1p-126f);  // never 0: a masked score of -inf stays one
           float own_sum = 0.f, own_top = -INFINITY;
-          const bool own = (wide[s * 4 + 2 * u] | wide[s * 4 + 2 * u + 1]) != 0;
+          const bool own = !kSplit && (wide[s * 4 + 2 * u] | wide[s * 4 + 2 * u + 1]) != 0;
           if (own) {
             // keys with exponents of their own: T_j - E takes the place of their scores, and the s_j are summed up here
             const uint32_t* sh = shift + s * 128 + u * 64;
@@ -397,7 +407,7 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
       }
     } else if (warp < 12) {
       // ------------------------------------------------ codes to operands: a thread a key
-      const int key = threadIdx.x - 256, part = warp - 8;
+      const int key = threadIdx.x - 256, part = warp - 8, odd = part >> 1;  // odd: its 64 keys of the tile
       uint4 kc[D / 32], vc[D / 32];
       uint32_t ka = 0, va = 0;
       bool have = false, lost = false;
@@ -444,16 +454,45 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
               make_uint4(two(w & kCode0, s24), two(w & kCode1, s20), two(u & kCode0, s24), two(u & kCode1, s20));
         }
       };
+      // the same in 32 bits, as the top 11 bits and the rest; 32 elements a turn (unrolled, the code alone would bind)
+      auto split = [&](uint8_t* dst, uint4 (&codes)[D / 32], float2 f, int x) {
+        const float st = 16.f * times_pow2(f.x, -x), lo = times_pow2(f.y, -x) - st;
+#pragma unroll 1
+        for (int c = 0; c < D / 8; c += 4) {
+          const uint32_t words[4] = {codes[0].x, codes[0].y, codes[0].z, codes[0].w};
+#pragma unroll
+          for (int i = 0; i + 1 < D / 32; ++i) codes[i] = codes[i + 1];
+          uint8_t* row = dst + (c >> 3) * C::kHalf + key * 128;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t w = words[k];
+            float hi[8], rest[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {  // code n in the top bits of 1 + n / 16
+              const uint32_t n = i < 5 ? w << (19 - 4 * i) : w >> (4 * i - 19);
+              const float y = fmaf(__uint_as_float((n & 0x00780000u) | 0x3f800000u), st, lo);
+              hi[i] = __uint_as_float(__float_as_uint(y) & 0xffffe000u);
+              rest[i] = y - hi[i];
+            }
+            uint8_t* to = row + ((((c + k) & 7) ^ (key & 7)) << 4);
+            *reinterpret_cast<uint4*>(to) = make_uint4(pack2<__half>(hi[0], hi[4]), pack2<__half>(hi[1], hi[5]),
+                                                       pack2<__half>(hi[2], hi[6]), pack2<__half>(hi[3], hi[7]));
+            *reinterpret_cast<uint4*>(to + C::kTile) =
+                make_uint4(pack2<__half>(rest[0], rest[4]), pack2<__half>(rest[1], rest[5]), pack2<__half>(rest[2], rest[6]),
+                           pack2<__half>(rest[3], rest[7]));
+          }
+        }
+      };
       look(0);
       load(0);
       look(1);
       bool ok = true;
       int run = -1000;  // the largest exponent of values so far
-      // the exponent that puts a largest element of x under 2^-6
-      auto exponent = [](float x) { return log2i(x) + 7; };
+      // the exponent that puts a largest element of x under 2^-6, split 2^15
+      auto exponent = [](float x) { return kSplit ? log2i(fmaxf(x, 0x1p-24f)) - 14 : log2i(x) + 7; };
       for (int t = 0; t < tiles; ++t) {
-        const int s = t & 1;
-        const uint32_t ph = (t >> 1) & 1u;
+        const int s = t & 1, st = stage_of(2 * t + odd);
+        const uint32_t use = use_of(2 * t + odd);
         float2 kf = unpack2<T>(ka), vf = unpack2<T>(va);
         const bool sick = !isfinite(vf.x) || !isfinite(vf.y);
         if (sick) vf = make_float2(0.f, 0.f);
@@ -470,39 +509,45 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
         if (lane == 0) tile_max[(s * 4 + part) * 2] = km, tile_max[(s * 4 + part) * 2 + 1] = vm;
         const unsigned gone = __ballot_sync(0xffffffffu, lost), ill = __ballot_sync(0xffffffffu, sick && have);
         // a warp whose wait ran out still comes here, so that none of the others stays behind
-        if (!named_bar_and(1, 128, ok)) break;
+        if (!named_bar_and(kSplit ? 1 + odd : 1, kSplit ? 64 : 128, ok)) break;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          km = fmaxf(km, tile_max[(s * 4 + i) * 2]);
-          vm = fmaxf(vm, tile_max[(s * 4 + i) * 2 + 1]);
+        for (int i = 1; i < (kSplit ? 2 : 4); ++i) {
+          km = fmaxf(km, tile_max[(s * 4 + (part ^ i)) * 2]);
+          vm = fmaxf(vm, tile_max[(s * 4 + (part ^ i)) * 2 + 1]);
         }
         const int kx = exponent(km), vx = exponent(vm);
         // keys far below the tile's largest have exponents of their own (zeros fit any)
-        auto apart = [&](float x, int tile) { return x > 0.f && tile - exponent(x) > 4 ? tile - exponent(x) : 0; };
+        auto apart = [&](float x, int tile) { return !kSplit && x > 0.f && tile - exponent(x) > 4 ? tile - exponent(x) : 0; };
         const int ksh = apart(kown, kx), vsh = apart(vown, vx);
         run = max(run, vx);
         const unsigned far = __ballot_sync(0xffffffffu, ksh | vsh || vx < run - 20);
         if (lost) raise_status(kStatusBadIndex);
 
-        ok = __all_sync(0xffffffffu, t < 2 || mbar_wait(&kempty[s], ph ^ 1u, abort_flag));
+        ok = __all_sync(0xffffffffu, use == 0 || mbar_wait(&kempty[st], (use & 1u) ^ 1u, abort_flag));
         if (!ok) continue;
-        expand(ks + s * C::kTile, kc, kf, kx - ksh);
+        if constexpr (kSplit)
+          split(ks, kc, kf, kx);
+        else
+          expand(ks + s * C::kTile, kc, kf, kx - ksh);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&kfull[s]);
-        ok = __all_sync(0xffffffffu, t < 2 || mbar_wait(&vempty[s], ph ^ 1u, abort_flag));
+        if (lane == 0) mbar_arrive(&kfull[st]);
+        ok = __all_sync(0xffffffffu, use == 0 || mbar_wait(&vempty[st], (use & 1u) ^ 1u, abort_flag));
         if (!ok) continue;
-        expand(vs + s * C::kTile, vc, vf, vx - vsh);
-        shift[s * 128 + key] = static_cast<uint32_t>(ksh) | static_cast<uint32_t>(vsh) << 16;
-        if (lane == 0) {  // the tile's facts: its stage's last user read them before its values were multiplied
+        if constexpr (kSplit)
+          split(vs, vc, vf, vx);
+        else
+          expand(vs + s * C::kTile, vc, vf, vx - vsh);
+        if constexpr (!kSplit) shift[s * 128 + key] = static_cast<uint32_t>(ksh) | static_cast<uint32_t>(vsh) << 16;
+        if (lane == 0) {  // the tile's facts: their last user read them before its values were multiplied
           hide[s * 4 + part] = gone;
           poison[s * 4 + part] = ill;
           wide[s * 4 + part] = far;
-          if (part == 0) kexp[s] = kx, vexp[s] = vx;
+          if (!(part & 1)) kexp[s * 2 + odd] = kx, vexp[s * 2 + odd] = vx;
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&vfull[s]);
+        if (lane == 0) mbar_arrive(&vfull[st]);
         load(t + 1);
         look(t + 2);
       }
@@ -513,47 +558,53 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
       const uint64_t v_desc = umma_desc_sw128_mn_atoms(smem_u32(vs), C::kHalf);
       // S of tile i, keys 64 sub ..: into its buffer sub & 1
       const int i = warp - 12;  // the tile
+      constexpr int kParts = kSplit ? 2 : 1;
+      // where the operands of keys 64 sub .. begin
+      auto keys_at = [&](int sub) {
+        return static_cast<uint32_t>(((kSplit ? 0 : stage_of(sub) * C::kTile) + (sub & 1) * 64 * 128) >> 4);
+      };
+      // whether no later keys of this stage's filling follow
+      auto last_of = [&](int sub) { return kSplit || (sub & 1) || sub + 1 == subs; };
       // S of keys 64 sub .. into its buffer sub & 1
       auto scores = [&](int sub) {
-        const int s = (sub >> 1) & 1, u = sub & 1;
+        const int st = stage_of(sub), u = sub & 1;
+        if (!__all_sync(0xffffffffu, mbar_wait(&kfull[st], use_of(sub) & 1u, abort_flag))) return false;
+        tc_fence_after();
         const uint64_t qd = q_desc + static_cast<uint32_t>(i * C::kTile >> 4);
-        const uint64_t kd = k_desc + static_cast<uint32_t>((s * C::kTile + u * 64 * 128) >> 4);
+        const uint64_t kd = k_desc + keys_at(sub);
         if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = static_cast<uint32_t>((k >> 2) * C::kHalf + (k & 3) * 32) >> 4;
-            umma_f16_ss(tmem + i * 128 + u * 64, qd + off, kd + off, id_qk, k > 0 ? 1u : 0u);
+          for (int k = 0; k < kParts * D / 16; ++k) {
+            const int part = k / (D / 16), in = k % (D / 16);
+            const uint32_t off = static_cast<uint32_t>((in >> 2) * C::kHalf + (in & 3) * 32) >> 4;
+            umma_f16_ss(tmem + i * 128 + u * 64, qd + off, kd + off + (part * C::kTile >> 4), id_qk, k > 0 ? 1u : 0u);
           }
           umma_commit(&sfull[2 * i + u]);
-          if (u == 1 || sub + 1 == subs) umma_commit(&kempty[s]);
+          if (last_of(sub)) umma_commit(&kempty[st]);
         }
         __syncwarp();
+        return true;
       };
-      bool ok = i < halves && mbar_wait(qfull, 0, abort_flag) && mbar_wait(&kfull[0], 0, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      tc_fence_after();
-      for (int sub = 0; ok && sub < min(subs, 2); ++sub) scores(sub);
+      bool ok = __all_sync(0xffffffffu, i < halves && mbar_wait(qfull, 0, abort_flag));
+      for (int sub = 0; ok && sub < min(subs, 2); ++sub) ok = scores(sub);
       for (int sub = 0; ok && sub < subs; ++sub) {
-        const int t = sub >> 1, u = sub & 1, s = t & 1;
-        const uint64_t vd = v_desc + static_cast<uint32_t>((s * C::kTile + u * 64 * 128) >> 4);
-        if (u == 0) {
-          ok = mbar_wait(&vfull[s], (t >> 1) & 1u, abort_flag) &&
-               (sub + 2 >= subs || mbar_wait(&kfull[s ^ 1], ((t + 1) >> 1) & 1u, abort_flag));
-        }
-        ok = ok && mbar_wait(&pfull[2 * i + u], t & 1u, abort_flag);
+        const int st = stage_of(sub), u = sub & 1;
+        const uint64_t vd = v_desc + keys_at(sub);
+        ok = mbar_wait(&vfull[st], use_of(sub) & 1u, abort_flag) &&
+             mbar_wait(&pfull[2 * i + u], (sub >> 1) & 1u, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + u * 64 + k * 8, vd + (k * 2048 >> 4), id_pv,
-                        sub > 0 || k > 0 ? 1u : 0u);
+          for (int k = 0; k < kParts * 4; ++k)
+            umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + u * 64 + k % 4 * 8,
+                        vd + ((k / 4 * C::kTile + k % 4 * 2048) >> 4), id_pv, sub > 0 || k > 0 ? 1u : 0u);
           umma_commit(&odone[2 * i + u]);
-          if (u == 1 || sub + 1 == subs) umma_commit(&vempty[s]);
+          if (last_of(sub)) umma_commit(&vempty[st]);
         }
         __syncwarp();
-        if (sub + 2 < subs) scores(sub + 2);
+        if (sub + 2 < subs) ok = scores(sub + 2);
       }
       if (elect_one()) umma_commit(&done[i]);
       mbar_wait(&done[i], 0, nullptr);  // nothing is in flight when the memory goes

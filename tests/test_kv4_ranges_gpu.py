@@ -163,6 +163,29 @@ def test_large_values_of_no_weight(cuda_device, dtype, mix, log2):
     check(bt, q, ops.kv4_attention(bt.cache, q, *bt.where))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_f16_prompts_are_exact_but_for_two_roundings(cuda_device, D):
+    """f16 prompts and chunks over keys with channels seven times the others. The output and the weights round to 11 bits, by
+    at most 2^-11 / sqrt(3) each in the mean square; independent, they add up to 2^-11 sqrt(2/3). All else is 32-bit."""
+    from dscquant_b200 import ops
+
+    g = torch.Generator(device=cuda_device).manual_seed(25)
+    bt = Batch([(300, 1500), (257, 2100)], 16, D, 64, torch.float16, cuda_device)
+    for b, (_, L) in enumerate(bt.seqs):
+        pages, off = bt.slots(b, 0, L)
+        loud = 1 + 6 * (torch.rand(1, 16, D, generator=g, device=cuda_device) < 0.03)
+        for side, by in (("k", loud), ("v", 1)):
+            y = torch.randn(L, 16, D, generator=g, device=cuda_device, dtype=torch.float64) * by
+            code, step, low = quantise(y, torch.float16)
+            getattr(bt.cache, side + "_codes")[pages, :, off] = pack(code)
+            getattr(bt.cache, side + "_affine")[pages, :, off] = torch.cat((step, low), -1).half()
+    q = randn((bt.T, 32, D), g, torch.float16)
+    ref = reference(bt, q)[0]
+    for max_q in (None, 300):
+        out = ops.kv4_attention(bt.cache, q, *bt.where, max_q=max_q).double()
+        assert float((out - ref).norm() / ref.norm()) <= 2.0 ** -11 * (2 / 3) ** 0.5 * 1.01
+
+
 @pytest.mark.parametrize("mix", [FEW, MANY], ids=["few", "many"])
 def test_rows_behind_the_page_table_are_zero(cuda_device, mix):
     """A length beyond what the page table holds: rows at positions behind it are left out (zero), the others stay."""
