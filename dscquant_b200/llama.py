@@ -178,7 +178,9 @@ class LlamaW4A4:
              lengths: torch.Tensor, max_q: int | None = None) -> torch.Tensor:
         """Logits [T, vocab] of new tokens ids [T] of a batch of sequences (described as for ops.kv4_append;
         `lengths` counts them in), which join the caches."""
-        cos, sin = self.rope(page_table.shape[1] * caches[0].page_size)
+        positions = max(page_table.shape[1] * caches[0].page_size, 1)
+        # tables are kept (captured steps read them) and of a power of two, so that page tables of all widths share a few
+        cos, sin = self.rope(1 << (positions - 1).bit_length())
         h = self.embed[ids]
         for layer, cache in zip(self.layers, caches):
             h = layer.step(h, cos, sin, cache, (page_table, q_start, lengths), max_q)
