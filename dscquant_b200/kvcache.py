@@ -59,4 +59,5 @@ class PagedKV4:
         return cls(codes[0], affine[0], codes[1], affine[1])
 
     def nbytes(self) -> int:
+        """Bytes of the cache's tensors: what a caller that sizes its page pool has to count."""
         return sum(t.numel() * t.element_size() for t in (self.k_codes, self.k_affine, self.v_codes, self.v_affine))
