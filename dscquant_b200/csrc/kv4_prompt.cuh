@@ -516,9 +516,10 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
           vm = fmaxf(vm, tile_max[(s * 4 + (part ^ i)) * 2 + 1]);
         }
         const int kx = exponent(km), vx = exponent(vm);
-        // keys far below the tile's largest have exponents of their own (zeros fit any)
+        // keys far below the tile's largest have exponents of their own; a seen value row of zeros has the lowest, so that its
+        // T_j moves no maximum
         auto apart = [&](float x, int tile) { return !kSplit && x > 0.f && tile - exponent(x) > 4 ? tile - exponent(x) : 0; };
-        const int ksh = apart(kown, kx), vsh = apart(vown, vx);
+        const int ksh = apart(kown, kx), vsh = !kSplit && vown == 0.f && have && !sick ? 254 : apart(vown, vx);
         run = max(run, vx);
         const unsigned far = __ballot_sync(0xffffffffu, ksh | vsh || vx < run - 20);
         if (lost) raise_status(kStatusBadIndex);

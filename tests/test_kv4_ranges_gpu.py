@@ -213,3 +213,45 @@ def test_rows_behind_the_page_table_are_zero(cuda_device, mix):
     assert bool(out[lo:lo + 2].any())
     err = (out[:lo + 2].float() - want.float()).abs()
     assert bool((err <= 2.0 ** -6 * want.float().abs() + 2.0 ** -8).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("mix", [FEW, MANY], ids=["few", "many"])
+def test_rows_of_every_size(cuda_device, dtype, D, mix):
+    """Each cached row of a size of its own (keys smaller than the queries' units, values either way), zero and constant rows
+    among them, then a value row that is no number and a page out of range."""
+    from dscquant_b200 import ops
+
+    seqs, heads, kv_heads = mix
+    g = torch.Generator(device=cuda_device).manual_seed(27)
+    bt = Batch(seqs, kv_heads, D, 16, dtype, cuda_device)
+    bt.fill(g, v_offset=0.3)
+    wide = 40 if dtype is torch.bfloat16 else 8
+
+    def exponents(lo, hi):
+        return torch.randint(lo, hi + 1, bt.cache.k_affine.shape[:3], generator=g, device=cuda_device)
+
+    for affine, by in ((bt.cache.k_affine, exponents(-wide, 0)), (bt.cache.v_affine, exponents(-wide, wide))):
+        a = torch.nan_to_num(affine.float()) * 2.0 ** by[..., None]
+        kind = exponents(0, 15)
+        a[..., 0] = torch.where(kind < 2, 0.0, a[..., 0])
+        a[..., 1] = torch.where(kind == 0, 0.0, a[..., 1])
+        affine.copy_(a.to(dtype))
+    q = randn((bt.T, heads, D), g, dtype)
+    want = ops.kv4_attention(bt.cache, q, *bt.where)
+    check(bt, q, want)
+    assert torch.equal(want, ops.kv4_attention(bt.cache, q, *bt.where))
+    n, L = seqs[-1]
+    pages, off = bt.slots(len(seqs) - 1, L - 2, L - 1)
+    kept = bt.cache.v_affine.clone()
+    bt.cache.v_affine[pages, :, off] = torch.nan
+    out = ops.kv4_attention(bt.cache, q, *bt.where)
+    sees = torch.zeros(bt.T, dtype=torch.bool, device=cuda_device)
+    sees[bt.starts[-1] - 2:] = True
+    assert torch.isnan(out[sees]).all() and torch.equal(out[~sees], want[~sees])
+    bt.cache.v_affine.copy_(kept)
+    bt.table[0, 1] = bt.pages
+    out = ops.kv4_attention(bt.cache, q, *bt.where)
+    assert ops.device_status(cuda_device) == 4
+    assert torch.isfinite(out).all() and torch.equal(out[bt.starts[1]:], want[bt.starts[1]:])
