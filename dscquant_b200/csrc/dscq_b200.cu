@@ -569,8 +569,14 @@ cudaError_t launch_kv4_attention(const dscq::Kv4AttnParams& a, int64_t max_q, vo
   const int64_t all = std::numeric_limits<int64_t>::max();
   const int64_t rows = max_q * a.group;
   if (rows <= 8) return launch_kv4_decode<T, D, 1>(a, all, ws, st);
-  // Sequences of more than 64 rows go to the tensor-core kernel, when there can be enough of them to fill
-  // a quarter of the GPU with CTAs of 256 rows.
+  // Sequences of more than 64 rows (tokens x query heads of a key head) go to the tensor-core kernel, when there can be
+  // enough of them to fill a quarter of the GPU with CTAs of 256 rows: that kernel takes a CTA's time whatever the number
+  // of CTAs, the shared-out one reads the cache once per 16 rows. Measured (bf16, heads of 128, us, shared-out |
+  // tensor cores; the same side wins at 1000 and 32000 keys):
+  //   64/8 heads, one sequence over 8000 keys, rows (CTAs): 512 (16) 115 | 188, 800 (32) 170 | 188, 1200 (40) 242 | 191
+  //   32/32 heads, one sequence over 8000: 100 (32) 104 | 156, 150 (32) 139 | 186, 300 (64) 242 | 191
+  //   32/32 heads, four sequences over 8000, rows of each: 32: 117 | 162, 64: 209 | 164, 100: 350 | 164
+  // f16, whose tensor-core products are split, breaks even later (32/32 heads, 300 rows, 64 CTAs: 250 | 256).
   const int64_t few = 64, all_rows = static_cast<int64_t>(a.T) * a.group;
   const int64_t ctas = (all_rows / 256 + std::min<int64_t>(a.b.B, all_rows / (few + 1))) * a.b.hk;
   if (rows <= few || (all_rows + 255) / 256 * a.b.hk < num_sms() / 4 || ctas >= (int64_t(1) << 31))
