@@ -14,8 +14,8 @@
 // element under 2^-6. That rounds keys and values to 11 bits; queries, scaled by a power of two a row, are exact. Scores,
 // statistics and sums are 32-bit.
 // For f16, whose outputs would show that rounding (7e-4 of the result against 64 bits instead of 3e-4), keys and values are
-// made in 32 bits and split into two fp16 parts, 21 bits, each multiplied: twice the products, and stages of 64 keys
-// instead of 128 for the same memory. The weights' rounding is the one that stays.
+// split into two fp16 parts, each multiplied, which together are within 2^-18 of a row's largest element: twice the
+// products, and stages of 64 keys instead of 128 for the same memory. The weights' rounding is the one that stays.
 //
 // What a row does not see, or hardly weighs, must not cost it bits. With s_j the score of key j and v_j = V_j 2^(E_j) its
 // scaled value row, the weights handed to the product are W_j = fp16(2^(T_j - M)), T_j = s_j + E_j, M a running maximum of
@@ -32,11 +32,13 @@
 // Keys no row may see (behind the end, on pages out of range) are zeros with their scores masked. A value row that is
 // not finite is zeros too and flagged; rows that see its key become NaN, the others must not.
 //
-// Measured on a B200: chunks of 1000 to 1500 rows over 8 to 10 thousand keys, 64 heads on 8: 933 us, 801 TFLOP/s (0.47 of
-// the cuBLAS rate); three prompts of 900 to 2048 tokens, 32 heads: 147 us. Without its products the kernel takes 912 us:
-// what binds is the softmax's own chain (read 64 scores, maximum, exponentials, write) and its handshakes, two
-// tiles' worth at a time; short prompts add 3 us of setting up and draining to each CTA's few tiles. One warp issuing both
-// tiles' products made the chunks 962 us.
+// Measured on a B200 (kernel, with its companion for short sequences): chunks of 1000 to 1500 rows over 8 to 10 thousand
+// keys, 64 heads on 8: bf16 997 us, 749 TFLOP/s (0.44 of the cuBLAS rate), f16 1180 us; three prompts of 900 to 2048 tokens,
+// 32 heads: bf16 151 us, f16 188 us. What binds is the softmax's own chain (read 64 scores, maximum, exponentials, write)
+// and its handshakes, two tiles' worth at a time, on 128 registers a thread: 14 warps leave no more, and at D = 128 120
+// bytes (f16 212) are spilled. For f16 it is the split of the codes besides: in 32 bits, leaving out half of it took 160 us
+// off, half of the products 33. Short prompts add 3 us of setting up and draining to each CTA's few tiles. One
+// warp issuing both tiles' products made the chunks 3% slower.
 //
 // Warps 0-3, 4-7: softmax of tile 0 and 1 (a thread a row); 8-11: codes to operands (split: 8, 9 the even, 10, 11 the odd
 // 64 keys, independently); 12, 13: the products of tile 0
@@ -454,9 +456,27 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
               make_uint4(two(w & kCode0, s24), two(w & kCode1, s20), two(u & kCode0, s24), two(u & kCode1, s20));
         }
       };
-      // the same in 32 bits, as the top 11 bits and the rest; 32 elements a turn (unrolled, the code alone would bind)
+      // The same in two parts, code * step_a + low_a and code * step_b + low_b. step_a and low_a are the multiples of g nearest to
+      // step and low, with g the power of two that makes every element less than 1024 g: the first part is exact, and
+      // the second, at most 8 g, rounds by 2^-18 of the row's largest element. (In 32 bits, ten instructions for two
+      // elements instead of five, chunks of 1000 to 1500 rows over 8k took 1.34 ms instead of 1.18.) 32 elements a
+      // turn: unrolled, the length of the code alone would bind.
       auto split = [&](uint8_t* dst, uint4 (&codes)[D / 32], float2 f, int x) {
-        const float st = 16.f * times_pow2(f.x, -x), lo = times_pow2(f.y, -x) - st;
+        const float st = times_pow2(f.x, -x), lo = times_pow2(f.y, -x);
+        const int e = max(log2i(fmaxf(fabsf(lo), fabsf(fmaf(15.f, st, lo)))), -30) - 9;
+        const float g = pow2f(e), per = pow2f(-e), sa = rintf(st * per) * g, la = rintf(lo * per) * g;
+        const __half2 sa2 = __float2half2_rn(sa), la2 = __float2half2_rn(la);
+        const __half2 sb2 = __float2half2_rn(st - sa), lb2 = __float2half2_rn(lo - la);
+        const __half2 zero = __float2half2_rn(1024.f);
+        auto two = [&](uint32_t w, uint32_t& hi, uint32_t& rest) {
+          w = (w & kCode0) | 0x64006400u;  // a code in the low bits of 1024
+          __half2 n;
+          memcpy(&n, &w, 4);
+          n = __hsub2(n, zero);
+          const __half2 h = __hfma2(n, sa2, la2), r = __hfma2(n, sb2, lb2);
+          memcpy(&hi, &h, 4);
+          memcpy(&rest, &r, 4);
+        };
 #pragma unroll 1
         for (int c = 0; c < D / 8; c += 4) {
           const uint32_t words[4] = {codes[0].x, codes[0].y, codes[0].z, codes[0].w};
@@ -465,21 +485,14 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
           uint8_t* row = dst + (c >> 3) * C::kHalf + key * 128;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t w = words[k];
-            float hi[8], rest[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {  // code n in the top bits of 1 + n / 16
-              const uint32_t n = i < 5 ? w << (19 - 4 * i) : w >> (4 * i - 19);
-              const float y = fmaf(__uint_as_float((n & 0x00780000u) | 0x3f800000u), st, lo);
-              hi[i] = __uint_as_float(__float_as_uint(y) & 0xffffe000u);
-              rest[i] = y - hi[i];
-            }
+            uint4 hi, rest;
+            two(words[k], hi.x, rest.x);
+            two(words[k] >> 4, hi.y, rest.y);
+            two(words[k] >> 8, hi.z, rest.z);
+            two(words[k] >> 12, hi.w, rest.w);
             uint8_t* to = row + ((((c + k) & 7) ^ (key & 7)) << 4);
-            *reinterpret_cast<uint4*>(to) = make_uint4(pack2<__half>(hi[0], hi[4]), pack2<__half>(hi[1], hi[5]),
-                                                       pack2<__half>(hi[2], hi[6]), pack2<__half>(hi[3], hi[7]));
-            *reinterpret_cast<uint4*>(to + C::kTile) =
-                make_uint4(pack2<__half>(rest[0], rest[4]), pack2<__half>(rest[1], rest[5]), pack2<__half>(rest[2], rest[6]),
-                           pack2<__half>(rest[3], rest[7]));
+            *reinterpret_cast<uint4*>(to) = hi;
+            *reinterpret_cast<uint4*>(to + C::kTile) = rest;
           }
         }
       };
