@@ -24,10 +24,10 @@
 // finishes runs that lie inside its share; pieces of cut runs meet in shared memory once all warps of the
 // CTA are done, pieces of runs cut by CTA borders in a second kernel, in order: no atomics, the same bits every time.
 //
-// Measured on a B200: 64 contexts of 0 to 8191 tokens, 64 heads on 8: 78 us for 287 MB (3.7 TB/s, 0.57 of the copy rate);
-// three of 50 to 65 thousand: 52 us (3.2 TB/s). Twelve warps an SM keep the issue slots half and the integer pipe two
-// thirds busy with the ANDs, permutes and copies of codes, and a tile's chain of products and exponentials does
-// not overlap further: 16 warps (32-key tiles, 128 registers) took 96 us, 8 warps 90, 12 with 32-key tiles 91.
+// Measured on a B200: 64 contexts of 0 to 8191 tokens, 64 heads on 8: 80 us for 287 MB (3.6 TB/s, 0.55 of the copy rate; 78
+// with one F for all rows); three of 50 to 65 thousand: 52 us (3.2 TB/s). Twelve warps an SM keep the issue slots and
+// the integer pipe half busy with the ANDs, permutes and copies of codes, and a tile's chain of products and exponentials
+// does not overlap further: 16 warps (32-key tiles, 128 registers) took 96 us, 8 warps 90, 12 with 32-key tiles 91.
 #pragma once
 #include "kv4_attention.cuh"
 #include "rotq_tc.cuh"

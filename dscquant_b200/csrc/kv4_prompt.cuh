@@ -22,19 +22,19 @@
 // the T_j that the row sees, and
 //   out = 2^M sum W_j V_j / sum 2^(s_j).
 // E_j is the tile's exponent, but for bf16 a key whose largest element is under 1/16 of the tile's has its own (and keys
-// their own scale likewise), so that fp16 keeps 2^-13 of every row's largest element at least. Tiles with such keys, and those whose exponent is 20 below an earlier one, so that
-// the sum of the 2^(s_j) cannot be had from the weights in 32 bits, are marked wide and take a slower path. (All of f16's
-// range fits two parts under one scale: the largest element goes under 2^15, and 2^-40 of it stays.) M is a whole
-// number and only moves when it would be passed by 2^8; then the row's sums in TMEM are scaled, by the warps that own
-// them. Weights keep 11 bits down to 2^-21 of the largest. (The slower path is a loop over TMEM: a second copy of the
-// unrolled one cost the other tiles 9% for its length alone.)
+// their own scale likewise), so that fp16 keeps 2^-13 of every row's largest element at least. Tiles with such keys, and
+// those whose exponent is 20 below an earlier one, so that the sum of the 2^(s_j) cannot be had from the weights in 32
+// bits, are marked wide and take a slower path. (All of f16's range fits two parts under one scale: the largest element
+// goes under 2^15, and 2^-40 of it stays.) M is a whole number and only moves when it would be passed by 2^8; then the
+// row's sums in TMEM are scaled, by the warps that own them. Weights keep 11 bits down to 2^-21 of the largest. (The slower
+// path is a loop over TMEM: a second copy of the unrolled one cost the other tiles 9% for its length alone.)
 //
 // Keys no row may see (behind the end, on pages out of range) are zeros with their scores masked. A value row that is
 // not finite is zeros too and flagged; rows that see its key become NaN, the others must not.
 //
-// Measured on a B200 (kernel, with its companion for short sequences): chunks of 1000 to 1500 rows over 8 to 10 thousand
-// keys, 64 heads on 8: bf16 997 us, 749 TFLOP/s (0.44 of the cuBLAS rate), f16 1180 us; three prompts of 900 to 2048 tokens,
-// 32 heads: bf16 151 us, f16 188 us. What binds is the softmax's own chain (read 64 scores, maximum, exponentials, write)
+// Measured on a B200 (with the launch for short sequences before it): chunks of 1000 to 1500 rows over 8 to 10 thousand
+// keys, 64 heads on 8: bf16 1000 us, 747 TFLOP/s (0.44 of the cuBLAS rate), f16 1180 us; three prompts of 900 to 2048
+// tokens, 32 heads: bf16 151 us, f16 188 us. What binds is the softmax's own chain (read 64 scores, maximum, exponentials, write)
 // and its handshakes, two tiles' worth at a time, on 128 registers a thread: 14 warps leave no more, and at D = 128 120
 // bytes (f16 212) are spilled. For f16 it is the split of the codes besides: in 32 bits, leaving out half of it took 160 us
 // off, half of the products 33. Short prompts add 3 us of setting up and draining to each CTA's few tiles. One
@@ -456,8 +456,8 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
               make_uint4(two(w & kCode0, s24), two(w & kCode1, s20), two(u & kCode0, s24), two(u & kCode1, s20));
         }
       };
-      // The same in two parts, code * step_a + low_a and code * step_b + low_b. step_a and low_a are the multiples of g nearest to
-      // step and low, with g the power of two that makes every element less than 1024 g: the first part is exact, and
+      // The same in two parts, code * step_a + low_a and code * step_b + low_b. step_a and low_a are the multiples of g
+      // nearest to step and low, with g the power of two that makes every element less than 1024 g: the first part is exact, and
       // the second, at most 8 g, rounds by 2^-18 of the row's largest element. (In 32 bits, ten instructions for two
       // elements instead of five, chunks of 1000 to 1500 rows over 8k took 1.34 ms instead of 1.18.) 32 elements a
       // turn: unrolled, the length of the code alone would bind.
@@ -529,9 +529,11 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
           vm = fmaxf(vm, tile_max[(s * 4 + (part ^ i)) * 2 + 1]);
         }
         const int kx = exponent(km), vx = exponent(vm);
-        // keys far below the tile's largest have exponents of their own; a seen value row of zeros has the lowest, so that its
-        // T_j moves no maximum
-        auto apart = [&](float x, int tile) { return !kSplit && x > 0.f && tile - exponent(x) > 4 ? tile - exponent(x) : 0; };
+        // keys far below the tile's largest have exponents of their own; a seen value row of zeros has the lowest, so that
+        // its T_j moves no maximum
+        auto apart = [&](float x, int tile) {
+          return !kSplit && x > 0.f && tile - exponent(x) > 4 ? tile - exponent(x) : 0;
+        };
         const int ksh = apart(kown, kx), vsh = !kSplit && vown == 0.f && have && !sick ? 254 : apart(vown, vx);
         run = max(run, vx);
         const unsigned far = __ballot_sync(0xffffffffu, ksh | vsh || vx < run - 20);

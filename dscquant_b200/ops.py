@@ -513,8 +513,9 @@ def kv4_attention(cache: PagedKV4, q: torch.Tensor, page_table: torch.Tensor, q_
     q [T, q_heads, D] of the cache's type, already rotated (kv4_append's result); the batch is described as for
     kv4_append, whose rows it must already hold. Query head h reads key head h // (q_heads // kv_heads), a row
     at position p the positions 0 .. p. `scale` defaults to D ** -0.5. `max_q` says how many rows the longest
-    sequence has in this call (default T); it only spares a launch. Rows of no sequence and rows at positions before the first or
-    behind the page table are zero. Positions behind it and pages out of range raise bit 2 of `device_status`."""
+    sequence has in this call (default T); it only spares a launch. Rows of no sequence and rows at positions before
+    the first or behind the page table are zero; positions behind it and pages out of range raise bit 2 of
+    `device_status`."""
     if q.dim() != 3:
         raise RuntimeError("q must be [T, heads, D]")
     T, heads, D = q.shape
