@@ -56,6 +56,8 @@ struct Kv4PromptParams {
 constexpr int kKv4PromptThreads = 14 * 32;
 constexpr int64_t kKv4AllRows = INT64_MAX;
 
+// A whole number; what 32 bits do not count singly any more stays in range.
+__device__ __forceinline__ int whole(float x) { return static_cast<int>(fminf(fmaxf(x, -0x1p28f), 0x1p28f)); }
 // x 2^e in two steps, for |e| up to 250.
 __device__ __forceinline__ float times_pow2(float x, int e) { return x * pow2f(e / 2) * pow2f(e - e / 2); }
 
@@ -258,7 +260,7 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
         const uint32_t s_at = tmem + half * 128 + lanes, o_at = tmem + 256 + half * 128 + lanes;
         const int lim = real ? sq.sees(tok) : INT_MAX;  // a row of nothing masks nothing
         float m = -INFINITY, l = 0.f;  // M, a whole number
-        int unit = -1000;              // sum 2^(s_j) = l 2^unit
+        int unit = -(1 << 29);         // sum 2^(s_j) = l 2^unit; lower than any score
         bool ok = true, nan = false;
         for (int sub = 0; sub < subs; ++sub) {
           const int t = sub >> 1, u = sub & 1, s = t & 1;
@@ -370,7 +372,7 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
           }
           // ---- the sum of 2^(s_j) is that of 2^(T_j - M + 7) in units of 2^base, where the keys share an exponent
           const float sum = own ? own_sum : (sums[0] + sums[1]) + (sums[2] + sums[3]);
-          int in = static_cast<int>(own ? own_top : base);
+          int in = whole(own ? own_top : base);
           if (mt == -INFINITY) in = unit;  // (a sum over nothing, 0 or NaN)
           const int to = max(unit, in);
           l = fmaf(l, pow2f(max(unit - to, -126)), sum * pow2f(max(in - to, -126)));
@@ -387,7 +389,7 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 1) kv4_prompt_kernel(const 
         if (__all_sync(0xffffffffu, ok)) {
           tc_fence_after();
           const float inv = nan ? __int_as_float(0x7fc00000) : l == 0.f ? 0.f : 1.f / l;
-          const int ev = m == -INFINITY ? 0 : min(max(static_cast<int>(m) - 7 - unit, -250), 250);
+          const int ev = m == -INFINITY ? 0 : min(max(whole(m) - 7 - unit, -250), 250);
           T* out = static_cast<T*>(a.out) + ((sq.q0 + static_cast<int64_t>(tok)) * a.hq + hd) * D;
 #pragma unroll
           for (int c = 0; c < D; c += 32) {

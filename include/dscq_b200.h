@@ -295,8 +295,8 @@ int64_t dscq_kv4_attention_workspace(int head_dim);
 /*
  * Causal attention of the rows of the token axis over the cache: out [T, q_heads, D] (contiguous) =
  * softmax(scale * q k^T) v over the positions up to the row's own, query head h reading key head
- * h / (q_heads / kv_heads). Rows of no sequence, and rows that see no key, are zero. Query elements of 2^105 and more
- * (bf16) leave the range that is kept. `max_q` is the most rows
+ * h / (q_heads / kv_heads). Rows of no sequence, and rows that see no key, are zero. Kept are scores up to 2^22 in size and
+ * query elements below 2^105. `max_q` is the most rows
  * any sequence has in this call (0: unknown); it decides which kernels run. `workspace` (16-byte aligned) is
  * scratch of this call until it has run: calls that may overlap on the GPU need one each.
  */

@@ -255,3 +255,24 @@ def test_rows_of_every_size(cuda_device, dtype, D, mix):
     out = ops.kv4_attention(bt.cache, q, *bt.where)
     assert ops.device_status(cuda_device) == 4
     assert torch.isfinite(out).all() and torch.equal(out[bt.starts[1]:], want[bt.starts[1]:])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("mix", [FEW, MANY], ids=["few", "many"])
+@pytest.mark.parametrize("key", [-8.0, 8.0, -250.0, 250.0])
+def test_scores_far_from_zero(cuda_device, dtype, mix, key):
+    """Scores of thousands, of either sign and all alike: every row is the mean of the values it sees."""
+    from dscquant_b200 import ops
+
+    seqs, heads, kv_heads = mix
+    g = torch.Generator(device=cuda_device).manual_seed(28)
+    bt = Batch(seqs, kv_heads, 64, 16, dtype, cuda_device)
+    bt.fill(g, v_offset=0.5)
+    bt.cache.k_affine[..., 0] = 0
+    bt.cache.k_affine[..., 1] = key
+    q = torch.full((bt.T, heads, 64), 31.0, dtype=dtype, device=cuda_device)
+    for scale in (None, 1.0):
+        out = ops.kv4_attention(bt.cache, q, *bt.where, scale=scale).double()
+        ref = reference(bt, q, scale)[0]
+        # equal weights, 11-bit values and a rounded output: elements of at most 5 by 2^-12 of the terms and half a step
+        assert bool(((out - ref).abs() <= 2.0 ** -11 * 5 + torch.finfo(dtype).eps / 2 * ref.abs()).all())
